@@ -211,6 +211,113 @@ unsafe extern "C" {
         stream: *mut Stream,
         error: *mut *mut c_char,
     ) -> i32;
+    pub fn vfr_layer_norm(
+        x: *const c_void,
+        gamma: *const f32,
+        beta: *const f32,
+        rows: i64,
+        width: i32,
+        dtype: i32,
+        eps: f32,
+        y: *mut c_void,
+        mean: *mut f32,
+        rstd: *mut f32,
+        packed: *mut u8,
+        exponents: *mut u8,
+        stream: *mut Stream,
+        error: *mut *mut c_char,
+    ) -> i32;
+    pub fn vfr_layer_norm_workspace(
+        rows: i64,
+        width: i32,
+        bytes: *mut usize,
+        error: *mut *mut c_char,
+    ) -> i32;
+    pub fn vfr_layer_norm_backward(
+        dy: *const c_void,
+        x: *const c_void,
+        packed: *const u8,
+        exponents: *const u8,
+        mean: *const f32,
+        rstd: *const f32,
+        gamma: *const f32,
+        rows: i64,
+        width: i32,
+        dtype: i32,
+        dx: *mut c_void,
+        dgamma: *mut f32,
+        dbeta: *mut f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: *mut Stream,
+        error: *mut *mut c_char,
+    ) -> i32;
+    pub fn vfr_checkpoint_pack(
+        x: *const c_void,
+        rows: i64,
+        width: i32,
+        dtype: i32,
+        packed: *mut u8,
+        exponents: *mut u8,
+        stream: *mut Stream,
+        error: *mut *mut c_char,
+    ) -> i32;
+    pub fn vfr_checkpoint_unpack(
+        packed: *const u8,
+        exponents: *const u8,
+        rows: i64,
+        width: i32,
+        dtype: i32,
+        x: *mut c_void,
+        stream: *mut Stream,
+        error: *mut *mut c_char,
+    ) -> i32;
+    pub fn vfr_unit_loss(
+        x: *const c_void,
+        units: *const c_void,
+        bias: *const f32,
+        labels: *const i32,
+        rows: i64,
+        k: i32,
+        width: i32,
+        dtype: i32,
+        scale: f32,
+        loss: *mut f32,
+        lse: *mut f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: *mut Stream,
+        error: *mut *mut c_char,
+    ) -> i32;
+    pub fn vfr_unit_loss_workspace(
+        rows: i64,
+        k: i32,
+        width: i32,
+        dtype: i32,
+        backward: i32,
+        bytes: *mut usize,
+        error: *mut *mut c_char,
+    ) -> i32;
+    pub fn vfr_unit_loss_backward(
+        x: *const c_void,
+        units: *const c_void,
+        bias: *const f32,
+        labels: *const i32,
+        lse: *const f32,
+        dloss: *const f32,
+        rows: i64,
+        k: i32,
+        width: i32,
+        dtype: i32,
+        scale: f32,
+        dx: *mut c_void,
+        dunits: *mut c_void,
+        dbias: *mut f32,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: *mut Stream,
+        error: *mut *mut c_char,
+    ) -> i32;
     pub fn vfr_ivf_build(
         centroids: *const f32,
         k: i32,

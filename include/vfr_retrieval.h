@@ -409,6 +409,83 @@ VFR_API int vfr_retrieval_search_sharded(VfrShardedIndex *index, const float *qu
 VFR_API int vfr_retrieval_blend_sharded(VfrShardedIndex *index, const float *queries, float *out, size_t frames,
                                         int32_t width, const float *index_rate, VfrStream *stream, char **error);
 
+/* ------------------------------------------------------------------------ */
+/* Training a content encoder's unit head                                   */
+/* ------------------------------------------------------------------------ */
+/* A content encoder is trained to tell a frame's unit: the k-means cluster
+ * (vfr_kmeans, vfr_ivf_assign) its features fall in.  The calls below are
+ * that head: layer norm of the frames, softmax cross entropy against a
+ * codebook of units, the gradients of both, and 8-bit checkpoints that keep
+ * an activation until the backward pass.  No counterpart in the reference.
+ *
+ * Matrices are row-major and contiguous, [rows][width] with width in
+ * 1..4096, of the element type `dtype`; pointers are memory of one device,
+ * on which the call runs whatever the current device, and outputs must not
+ * overlap inputs.  The calls are asynchronous on `stream` (stream->stream
+ * may be the default stream), allocate nothing, can be captured into CUDA
+ * graphs, and give the same bits every time.  A workspace is read and
+ * written until the call's work on the stream is done; calls that may run at
+ * the same time need one each. */
+enum { VFR_F32 = 0, VFR_BF16 = 1, VFR_F16 = 2 };
+
+/* mean = sum x / width, rstd = (sum (x - mean)^2 / width + eps)^(-1/2) and
+ * y = (x - mean) rstd gamma + beta per row; gamma, beta: f32 [width], either
+ * may be NULL; mean, rstd: f32 [rows].  With packed and exponents (both or
+ * neither) the same pass writes x's checkpoint, as vfr_checkpoint_pack. */
+VFR_API int vfr_layer_norm(const void *x, const float *gamma, const float *beta, int64_t rows, int32_t width,
+                           int32_t dtype, float eps, void *y, float *mean, float *rstd, uint8_t *packed,
+                           uint8_t *exponents, VfrStream *stream, char **error);
+/* Workspace bytes of vfr_layer_norm_backward on the current device. */
+VFR_API int vfr_layer_norm_workspace(int64_t rows, int32_t width, size_t *bytes, char **error);
+/* dx [rows][width] of `dtype`, and dgamma, dbeta (f32 [width], either may be
+ * NULL) from dy and the forward pass's input x, or its checkpoint (packed,
+ * exponents; x NULL).  gamma may be NULL.  workspace: 16-byte aligned, not
+ * needed without dgamma and dbeta.  rows = 0 writes zero dgamma and dbeta. */
+VFR_API int vfr_layer_norm_backward(const void *dy, const void *x, const uint8_t *packed, const uint8_t *exponents,
+                                    const float *mean, const float *rstd, const float *gamma, int64_t rows,
+                                    int32_t width, int32_t dtype, void *dx, float *dgamma, float *dbeta,
+                                    void *workspace, size_t workspace_bytes, VfrStream *stream, char **error);
+
+/* 8-bit checkpoint of x: e4m3 bytes packed [rows][width], and one byte
+ * s + 127 per 128 elements of a row, exponents [rows][ceil(width / 128)].
+ * 2^s is the smallest power of two (s >= -127) that brings the block's
+ * largest finite magnitude to at most 448; each element is rounded to
+ * nearest even as x / 2^s (error at most 2^-4 of it, or 2^(s - 10) where
+ * that is more).  Infinities and NaN are kept as NaN. */
+VFR_API int vfr_checkpoint_pack(const void *x, int64_t rows, int32_t width, int32_t dtype, uint8_t *packed,
+                                uint8_t *exponents, VfrStream *stream, char **error);
+/* The values a checkpoint stands for, rounded to `dtype` (exact in f32, but
+ * for magnitudes from 1.9375 * 2^127 on, which were rounded to 2^128). */
+VFR_API int vfr_checkpoint_unpack(const uint8_t *packed, const uint8_t *exponents, int64_t rows, int32_t width,
+                                  int32_t dtype, void *x, VfrStream *stream, char **error);
+
+/* Softmax cross entropy over k units: z[v] = scale x . units[v] + bias[v],
+ * lse = log sum_v exp z[v], loss = lse - z[label] per row, without keeping
+ * the logits.  x [rows][width], units [k][width]: VFR_F32 or VFR_BF16;
+ * bias: f32 [k] or NULL; labels: i32 [rows]; loss, lse: f32 [rows].  A label
+ * outside [0, k) is none: loss 0, no gradient, whatever the frame holds.  A
+ * unit whose bias is -inf takes no part and gets no gradient, whatever its
+ * row holds (a label on it: loss +inf); when all are, lse is -inf.  With vfr_kmeans centroids c, a
+ * bias of -scale |c|^2 / 2 gives the soft nearest-centroid choice.
+ * workspace: 256-byte aligned; f32 products are exact to 24 bits. */
+VFR_API int vfr_unit_loss(const void *x, const void *units, const float *bias, const int32_t *labels, int64_t rows,
+                          int32_t k, int32_t width, int32_t dtype, float scale, float *loss, float *lse,
+                          void *workspace, size_t workspace_bytes, VfrStream *stream, char **error);
+/* Workspace bytes of vfr_unit_loss (backward = 0) or vfr_unit_loss_backward
+ * (backward != 0) on the current device. */
+VFR_API int vfr_unit_loss_workspace(int64_t rows, int32_t k, int32_t width, int32_t dtype, int32_t backward,
+                                    size_t *bytes, char **error);
+/* Gradients from the forward pass's lse and dloss (f32 [rows], the gradient
+ * of each row's loss): dx [rows][width], dunits [k][width] of `dtype`, dbias
+ * f32 [k] or NULL, with G = dloss (exp(z - lse) - [v == label]): dx = scale
+ * G units, dunits = scale G^T x, dbias = column sums of G.  The logits are
+ * formed again, a piece of the units at a time.  rows = 0 writes zero dunits
+ * and dbias. */
+VFR_API int vfr_unit_loss_backward(const void *x, const void *units, const float *bias, const int32_t *labels,
+                                   const float *lse, const float *dloss, int64_t rows, int32_t k, int32_t width,
+                                   int32_t dtype, float scale, void *dx, void *dunits, float *dbias,
+                                   void *workspace, size_t workspace_bytes, VfrStream *stream, char **error);
+
 /* Self-test of the bounded wait every mbarrier wait in the library's kernels
  * uses (no counterpart in the reference): one thread waits on a barrier that
  * only `arrive` != 0 completes, giving up after limit_ns (at most 2 s).

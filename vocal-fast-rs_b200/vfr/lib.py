@@ -120,6 +120,18 @@ def load_library(path: str | None = None):
         "vfr_peer_rows_close": ([vp], None),
         "vfr_blend_peer": ([vp, vp, vp, vp, vp, sz, i32, vp, P(Stream), err], ctypes.c_int),
         "vfr_selftest_bounded_wait": ([ctypes.c_uint64, i32, P(i32), P(ctypes.c_uint64), err], ctypes.c_int),
+        "vfr_layer_norm": ([vp, vp, vp, i64, i32, i32, ctypes.c_float, vp, vp, vp, vp, vp, P(Stream), err],
+                           ctypes.c_int),
+        "vfr_layer_norm_workspace": ([i64, i32, P(sz), err], ctypes.c_int),
+        "vfr_layer_norm_backward": ([vp, vp, vp, vp, vp, vp, vp, i64, i32, i32, vp, vp, vp, vp, sz, P(Stream), err],
+                                    ctypes.c_int),
+        "vfr_checkpoint_pack": ([vp, i64, i32, i32, vp, vp, P(Stream), err], ctypes.c_int),
+        "vfr_checkpoint_unpack": ([vp, vp, i64, i32, i32, vp, P(Stream), err], ctypes.c_int),
+        "vfr_unit_loss": ([vp, vp, vp, vp, i64, i32, i32, i32, ctypes.c_float, vp, vp, vp, sz, P(Stream), err],
+                          ctypes.c_int),
+        "vfr_unit_loss_workspace": ([i64, i32, i32, i32, i32, P(sz), err], ctypes.c_int),
+        "vfr_unit_loss_backward": ([vp, vp, vp, vp, vp, vp, i64, i32, i32, i32, ctypes.c_float, vp, vp, vp, vp, sz,
+                                    P(Stream), err], ctypes.c_int),
         "vfr_retrieval_create_sharded": ([i32, P(i32), i32, i32, i32, i32, sz, vp, sz, vp, sz, vp, sz, vp, sz,
                                           P(Options), P(vp), err], ctypes.c_int),
         "vfr_retrieval_destroy_sharded": ([vp], None),
