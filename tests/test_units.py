@@ -182,12 +182,13 @@ def check_loss_grad(name, x, units, labels, lse, dloss, scale, bias, dx, dunits,
     finite_lse = lse.double().abs().nan_to_num(posinf=0.0, neginf=0.0)[:, None]
     dz = (6 * width + 32) * 2 * U * size + 4 * U * finite_lse
     half = HALF["bf16"] if name == "bf16" else 2 * U
-    eg = p * (dz + 8 * U) + g * (half + 2 * U)
+    under = 2.0 ** -126 * (1 + dloss.double().abs().nan_to_num())[:, None]
+    eg = p * (dz + 8 * U) + g * (half + 2 * U) + under
     tiny = 1e-36
     _within(dx, rdx, abs(scale) * ((eg + (6 * k + 16) * 2 * U * g) @ wa) + HALF[name] * rdx.abs() + tiny)
     _within(dunits, rdw, abs(scale) * ((eg + (6 * rows + 16) * 2 * U * g).t() @ xa) + HALF[name] * rdw.abs() + tiny)
     if bias is not None:
-        eb = p * (dz + 8 * U) + 2 * U * g
+        eb = p * (dz + 8 * U) + 2 * U * g + under
         _within(dbias, rdb, (eb + (rows + 16) * U * g).sum(0) + tiny)
 
 

@@ -82,6 +82,34 @@ __device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, u
         : "memory");
 }
 
+// 3-D tiled load, as tma_load_2d.
+__device__ __forceinline__ void tma_load_3d(void *dst, const CUtensorMap *map, uint64_t *bar, int32_t x, int32_t y,
+                                            int32_t z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+// 3-D tiled store from shared memory at non-negative coordinates (x a
+// multiple of 16 bytes); what lies outside the tensor is not written.  Part
+// of this thread's current bulk group.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, const void *src, int32_t x, int32_t y,
+                                             int32_t z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// All but the last kLeft groups of this thread have read their shared memory.
+template <int kLeft>
+__device__ __forceinline__ void bulk_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kLeft) : "memory");
+}
+// Every group of this thread has written global memory.
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // Untiled bulk copy of `bytes` from global memory into this CTA's shared
 // memory, completing `bar`'s transaction count.  Both addresses 16-byte
 // aligned, `bytes` a multiple of 16.
@@ -201,6 +229,22 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t smem_addr) {
     d |= 2ull << 61;
     return d;
 }
+
+// The same for an MN-major tile: per 64 elements of M (or N) one run of K
+// rows of 128 B (8-row atoms of 1024 B along K), the next 64 elements
+// `run_bytes` further: leading byte offset run_bytes, stride byte offset
+// 1024 B between 8-row groups along K.  16 K rows are 2048 B.
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t smem_addr, uint32_t run_bytes) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>((run_bytes >> 4) & 0x3FFFu) << 16;
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= 1ull << 46;
+    d |= 2ull << 61;
+    return d;
+}
+// idesc_f16 bits of an MN-major A or B operand.
+constexpr uint32_t kIdescMnA = 1u << 15, kIdescMnB = 1u << 16;
 
 // Instruction descriptor, kind::f16: D f32 (bits 4-5 = 1), A/B format in
 // bits 7-9 / 10-12 (0 = f16, 1 = bf16), both K-major, N >> 3 in bits 17-22,
