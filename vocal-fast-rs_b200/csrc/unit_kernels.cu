@@ -34,14 +34,17 @@ namespace {
 
 constexpr int kTileM = 128;      // TMEM lanes
 constexpr int kBlockK = 64;      // bf16 elements of one 128-byte swizzled row
-constexpr int kBox = 64;         // rows of every load's box
-constexpr uint32_t kBoxBytes = kBox * kBlockK * 2;
+constexpr uint32_t kBoxBytes = 64 * kBlockK * 2;  // 64 rows of 128 B
 constexpr int kEpiWarps = 8;     // two per lane quarter, each on half of a tile's columns
-constexpr int kThreads = 64 + 32 * kEpiWarps;  // warp 0 loads, warp 1 issues MMAs
+constexpr int kFirstEpi = 4;     // warps 0 and 2 load A and B, warp 1 issues MMAs, warp 3 only gives up registers
+constexpr int kThreads = 32 * (kFirstEpi + kEpiWarps);
+// 384 threads launch with 168 registers each: 64,512 = 128 x 72 + 256 x 216.
+constexpr int kRoleRegisters = 72, kEpiRegisters = 216;
+static_assert(128 * kRoleRegisters + 32 * kEpiWarps * kEpiRegisters <= 384 * 168, "register split");
 constexpr int kGroupM = 16;      // row tiles that share the units they read
 constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // 2^v by the hardware's approximation (2 units in the last place of f32 for
 // the arguments here, which are not above 0 but by rounding; results below
@@ -49,6 +52,32 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float exp2_approx(float v) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// Two f32 operations at a time.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "add.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "mul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return r;
 }
 
@@ -60,27 +89,32 @@ struct Shape {
     static constexpr int kTileN = kTerms == 1 ? 256 : 128;
     static constexpr int kStages = kTerms == 1 ? 4 : 2;
     static constexpr uint32_t kABytes = 2 * kBoxBytes;
-    static constexpr uint32_t kBBytes = kTileN / kBox * kBoxBytes;
+    static constexpr uint32_t kBBytes = kTileN / 64 * kBoxBytes;
     static constexpr uint32_t kStageBytes = kTerms * (kABytes + kBBytes);
     static constexpr uint32_t kStagingOff = kStages * kStageBytes;
     static constexpr uint32_t kBiasOff = kStagingOff + kEpiWarps * 2048;
-    static constexpr uint32_t kBarOff = kBiasOff + kEpiWarps * 128;
+    static constexpr uint32_t kBarOff = kBiasOff + kEpiWarps * kTileN / 2 * 4;
     static constexpr size_t kSmem = 1024 + kBarOff + 256;
-    // Depth blocks summed in tensor memory before f32 registers take over:
-    // the accumulator truncates, so f32 results add up short runs.
-    static constexpr int kChunk = kTerms == 1 ? 1 << 30 : 8;
     static_assert(kSmem <= 232448, "shared memory");
 };
 
 // A tile of a product: rows m0.., columns n0.. (n_cols of them, a multiple of
-// 16), depth blocks [k0, k1).  K-major operands are loaded at (k, row),
-// MN-major ones at (row, k).
+// 16), depth blocks [k0, k1).  One load brings a block of an operand's term:
+// K-major ones are boxes of 64 k by the tile's rows, at (k, row, 0, term);
+// MN-major ones 64 columns by 64 k, for each 64 columns of the tile, at
+// (0, k, column / 64, term).
 struct Tile {
     const CUtensorMap *a, *b;
     bool a_mn, b_mn;
-    int32_t m0, n0, n_cols, a_boxes;
+    int32_t m0, n0, n_cols;
     int32_t k0, k1;
 };
+
+// Depth blocks summed in tensor memory before f32 registers take over.  The
+// accumulator truncates where f32 rounds, which at depth 768 in one run puts
+// a bias of 1e-5 on a log-sum of 20; runs of 4 blocks leave a third of it.
+// Results that are rounded to bf16 anyway take one run.
+constexpr int kShortRun = 4, kOneRun = 1 << 30;
 
 struct Bars {
     uint64_t *full, *empty, *acc_full, *acc_empty;
@@ -101,43 +135,43 @@ __device__ __forceinline__ Bars bars_at(uint8_t *smem) {
     return b;
 }
 
-// Producer lane: every tile's operand blocks through the stages.  `tile(i, t)`
-// gives the CTA's i-th tile, false past the last.
-template <int kTerms, class TileAt>
-__device__ __forceinline__ void produce(uint8_t *smem, const Bars &bars, TileAt tile) {
+// A loading lane: its operand's blocks of every tile through the stages.  The
+// two operands have a lane each: one lane issues a load in some 170 cycles,
+// and a stage's MMAs take 512.  `walk.next` gives the CTA's next tile, false
+// past the last.
+template <int kTerms, bool kB, class Walk>
+__device__ __forceinline__ void produce(uint8_t *smem, const Bars &bars, Walk walk) {
     using S = Shape<kTerms>;
+    constexpr uint32_t kBytes = kB ? S::kBBytes : S::kABytes;
+    const uint32_t bytes = kTerms * (kB ? walk.a.tile_n * kBlockK * 2 : S::kABytes);
+    smem += kB ? kTerms * S::kABytes : 0;
     int stage = 0;
     uint32_t phase = 0;
-    Tile t;
-    for (int64_t i = 0; tile(i, t) && !*bars.abort_flag; ++i) {
-        const int b_boxes = (t.n_cols + kBox - 1) / kBox;
-        const uint32_t bytes = kTerms * (t.a_boxes + b_boxes) * kBoxBytes;
+    Tile t, after;
+    bool more = walk.next(t);
+    while (more && !*bars.abort_flag) {
+        const CUtensorMap *map = kB ? t.b : t.a;
+        const bool mn = kB ? t.b_mn : t.a_mn;
+        const int32_t r = kB ? t.n0 : t.m0;
         for (int k = t.k0; k < t.k1; ++k) {
             if (!tc::mbar_wait(&bars.empty[stage], phase ^ 1, kWaitLimitNs)) {
                 *bars.abort_flag = 1;
                 break;
             }
             tc::mbar_arrive_expect_tx(&bars.full[stage], bytes);
-            uint8_t *sa = smem + stage * S::kStageBytes, *sb = sa + kTerms * S::kABytes;
+            uint8_t *dst = smem + stage * S::kStageBytes;
             const int32_t kk = k * kBlockK;
 #pragma unroll
-            for (int p = 0; p < kTerms; ++p) {
-                for (int j = 0; j < t.a_boxes; ++j) {
-                    const int32_t r = t.m0 + j * kBox;
-                    tc::tma_load_3d(sa + p * S::kABytes + j * kBoxBytes, t.a, &bars.full[stage], t.a_mn ? r : kk,
-                                    t.a_mn ? kk : r, p);
-                }
-                for (int j = 0; j < b_boxes; ++j) {
-                    const int32_t r = t.n0 + j * kBox;
-                    tc::tma_load_3d(sb + p * S::kBBytes + j * kBoxBytes, t.b, &bars.full[stage], t.b_mn ? r : kk,
-                                    t.b_mn ? kk : r, p);
-                }
-            }
+            for (int p = 0; p < kTerms; ++p)
+                tc::tma_load_4d(dst + p * kBytes, map, &bars.full[stage], mn ? 0 : kk, mn ? kk : r, mn ? r / 64 : 0,
+                                p);
             if (++stage == S::kStages) {
                 stage = 0;
                 phase ^= 1;
             }
+            if (k == t.k0) more = walk.next(after);  // while this tile's copies are on their way
         }
+        t = after;
     }
     // let every issued copy land before the CTA can exit
     for (int s = 0; s < S::kStages; ++s) {
@@ -149,20 +183,24 @@ __device__ __forceinline__ void produce(uint8_t *smem, const Bars &bars, TileAt 
     }
 }
 
-// MMA lane.  Accumulator buffer b of a chunk: TMEM columns 256 b (the
-// product, or hi hi) and 256 b + 128 (the other terms' products).
-template <int kTerms, class TileAt>
-__device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32_t tmem, TileAt tile) {
+// MMA lane.  Accumulator buffer b of a run: TMEM columns 256 b (the product,
+// or hi hi) and 256 b + 128 (the other terms' products).
+template <int kTerms, int kRun, class Walk>
+__device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32_t tmem, Walk walk) {
     using S = Shape<kTerms>;
     int stage = 0;
     uint32_t phase = 0, acc_count = 0;
-    Tile t;
-    for (int64_t i = 0; tile(i, t) && !*bars.abort_flag; ++i) {
+    Tile t, after;
+    bool more = walk.next(t);
+    while (more && !*bars.abort_flag) {
         const uint32_t idesc = tc::idesc_f16(kTileM, t.n_cols, 1) | (t.a_mn ? tc::kIdescMnA : 0) |
                                (t.b_mn ? tc::kIdescMnB : 0);
-        const uint32_t a_step = t.a_mn ? 2048 : 32, b_step = t.b_mn ? 2048 : 32;
+        // descriptors of an operand at shared address 0, and their step (in 16 B) per 16 of depth
+        const uint64_t a_base = t.a_mn ? tc::smem_desc_sw128_mn(0, kBoxBytes) : tc::smem_desc_sw128(0);
+        const uint64_t b_base = t.b_mn ? tc::smem_desc_sw128_mn(0, kBoxBytes) : tc::smem_desc_sw128(0);
+        const uint32_t a_step = t.a_mn ? 2048 >> 4 : 32 >> 4, b_step = t.b_mn ? 2048 >> 4 : 32 >> 4;
         for (int k = t.k0; k < t.k1;) {
-            const int chunk = t.k1 - k > S::kChunk ? k + S::kChunk : t.k1;
+            const int stop = t.k1 - k > kRun ? k + kRun : t.k1;
             const uint32_t b = acc_count & 1;
             if (!tc::mbar_wait(&bars.acc_empty[b], ((acc_count >> 1) & 1) ^ 1, kWaitLimitNs)) {
                 *bars.abort_flag = 1;
@@ -171,7 +209,7 @@ __device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32
             tc::tc_fence_after();
             const uint32_t d = tmem + b * 256;
             uint32_t big = 0, rest = 0;  // whether each accumulator holds a sum
-            for (; k < chunk; ++k) {
+            for (; k < stop; ++k) {
                 if (!tc::mbar_wait(&bars.full[stage], phase, kWaitLimitNs)) {
                     *bars.abort_flag = 1;
                     return;
@@ -179,14 +217,11 @@ __device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32
                 tc::tc_fence_after();
                 const uint32_t sa = tc::smem_u32(smem + stage * S::kStageBytes), sb = sa + kTerms * S::kABytes;
                 auto product = [&](uint32_t acc, int pa, int pb, uint32_t &held) {
+                    const uint64_t da = a_base + ((sa + pa * S::kABytes) >> 4);
+                    const uint64_t db = b_base + ((sb + pb * S::kBBytes) >> 4);
 #pragma unroll
                     for (int kk = 0; kk < kBlockK / 16; ++kk) {
-                        const uint32_t xa = sa + pa * S::kABytes + kk * a_step;
-                        const uint32_t xb = sb + pb * S::kBBytes + kk * b_step;
-                        tc::mma_f16(acc,
-                                    t.a_mn ? tc::smem_desc_sw128_mn(xa, kBoxBytes) : tc::smem_desc_sw128(xa),
-                                    t.b_mn ? tc::smem_desc_sw128_mn(xb, kBoxBytes) : tc::smem_desc_sw128(xb), idesc,
-                                    held);
+                        tc::mma_f16(acc, da + kk * a_step, db + kk * b_step, idesc, held);
                         held = 1;
                     }
                 };
@@ -205,77 +240,59 @@ __device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32
                     stage = 0;
                     phase ^= 1;
                 }
+                if (k == t.k0) more = walk.next(after);  // while the tensor cores work
             }
             tc::mma_commit(&bars.acc_full[b]);
             ++acc_count;
         }
+        t = after;
     }
 }
 
-// Epilogue warps: `take(j, v)` gives this lane's row, columns 32 j .. of the
-// warp's half of the tile; all NaN once a wait gave up, so that no result of
-// a call that went wrong looks like one.
-template <int kTerms>
+// Epilogue warps: `load` leaves in v this lane's row of the warp's half of
+// the tile, 32 `chunks` columns of it; all NaN once a wait gave up, so that no
+// result of a call that went wrong looks like one.  The accumulator is free
+// again as soon as it is in registers.
+template <int kTerms, int kRun>
 struct Columns {
-    using S = Shape<kTerms>;
-    static constexpr int kMax = S::kTileN / 2 / 32;  // 32-column chunks of a half
-    float run[kTerms == 1 ? 1 : S::kTileN / 2];
+    static constexpr int kMax = Shape<kTerms>::kTileN / 2 / 32;  // 32-column chunks of a half
+    float v[kMax][32];
     uint32_t acc_count = 0;
     bool bad = false;
 
-    // Waits for the tile's accumulator (f32: adds up the tile's chunks).
-    __device__ __forceinline__ void open(const Bars &bars, uint32_t tmem, uint32_t half_at, int chunks, int depth) {
-        if constexpr (kTerms == 1) {
-            wait(bars);
-        } else {
+    // All kMax chunks are read, those past a narrow tile's too: their columns
+    // exist and nobody uses them.
+    __device__ __forceinline__ void load(const Bars &bars, uint32_t tmem, uint32_t half_at, int depth) {
+        uint32_t at = wait(bars, tmem + half_at);
 #pragma unroll
-            for (int i = 0; i < S::kTileN / 2; ++i) run[i] = 0.0f;
-            for (int k = 0; k < depth; k += S::kChunk) {
-                wait(bars);
-                const uint32_t at = tmem + half_at + (acc_count & 1) * 256;
+        for (int j = 0; j < kMax; ++j) tc::tmem_ld32_nowait(at + 32 * j, v[j]);
 #pragma unroll
-                for (int j = 0; j < kMax; ++j) {
-                    if (j < chunks) {
-                        float v[32];
-                        if (!bad) tc::tmem_ld32(at + 32 * j + 128, v);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) run[32 * j + i] += v[i];
-                        if (!bad) tc::tmem_ld32(at + 32 * j, v);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) run[32 * j + i] += v[i];
-                    }
-                }
-                release(bars);
-            }
+        for (int j = 0; j < kMax; ++j) tc::tmem_wait_ld32(v[j]);
+        if constexpr (kTerms > 1) add_from(at + 128);
+        release(bars);
+        while (kRun != kOneRun && (depth -= kRun) > 0) {
+            at = wait(bars, tmem + half_at);
+            if constexpr (kTerms > 1) add_from(at + 128);
+            add_from(at);
+            release(bars);
         }
-    }
-    __device__ __forceinline__ void take(uint32_t tmem, uint32_t half_at, int j, float (&v)[32]) {
-        if constexpr (kTerms == 1) {
-            if (!bad) tc::tmem_ld32(tmem + half_at + (acc_count & 1) * 256 + 32 * j, v);
-        } else {
+        if (bad) {
 #pragma unroll
-            for (int c = 0; c < kMax; ++c)
-                if (c == j)
+            for (int j = 0; j < kMax; ++j)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = run[32 * c + i];
+                for (int i = 0; i < 32; ++i) v[j][i] = NAN;
         }
-        if (bad)
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = NAN;
-    }
-    // The tile's last chunk has been taken.
-    __device__ __forceinline__ void close(const Bars &bars) {
-        if constexpr (kTerms == 1) release(bars);
     }
 
 private:
-    __device__ __forceinline__ void wait(const Bars &bars) {
+    __device__ __forceinline__ uint32_t wait(const Bars &bars, uint32_t base) {
         if (!bad && !tc::mbar_wait(&bars.acc_full[acc_count & 1], (acc_count >> 1) & 1, kWaitLimitNs)) {
             *bars.abort_flag = 1;
             bad = true;
         }
         bad = __any_sync(0xFFFFFFFFu, bad);
         tc::tc_fence_after();
+        return base + (acc_count & 1) * 256;
     }
     __device__ __forceinline__ void release(const Bars &bars) {
         tc::tc_fence_before();
@@ -283,12 +300,25 @@ private:
         if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&bars.acc_empty[acc_count & 1]);
         ++acc_count;
     }
+    __device__ __forceinline__ void add_from(uint32_t at) {
+#pragma unroll
+        for (int j = 0; j < kMax; ++j) {
+            float u[32];
+            tc::tmem_ld32_nowait(at + 32 * j, u);
+            tc::tmem_wait_ld32(u);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+                const float2 s = add2(make_float2(v[j][i], v[j][i + 1]), make_float2(u[i], u[i + 1]));
+                v[j][i] = s.x, v[j][i + 1] = s.y;
+            }
+        }
+    }
 };
 
 // The kernel around the roles: barriers, TMEM, and the epilogue
 // `epi(smem, bars, tmem, warp of the epilogue, lane)`.
-template <int kTerms, class TileAt, class Epi>
-__device__ __forceinline__ void run_roles(TileAt tile, Epi epi) {
+template <int kTerms, int kRun, class Walk, class Epi>
+__device__ __forceinline__ void run_roles(const Walk &walk, Epi epi) {
     using S = Shape<kTerms>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -297,7 +327,7 @@ __device__ __forceinline__ void run_roles(TileAt tile, Epi epi) {
     launch_dependents();
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
-            tc::mbar_init(&bars.full[s], 1);
+            tc::mbar_init(&bars.full[s], 2);
             tc::mbar_init(&bars.empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -316,13 +346,14 @@ __device__ __forceinline__ void run_roles(TileAt tile, Epi epi) {
     tc::tc_fence_after();
     const uint32_t tmem = *bars.tmem_slot;
     grid_dependency_wait();
-    if (warp == 0) {
-        if (lane == 0) produce<kTerms>(smem, bars, tile);
-        __syncwarp();
-    } else if (warp == 1) {
-        if (lane == 0) multiply<kTerms>(smem, bars, tmem, tile);
+    if (warp < kFirstEpi) {
+        tc::registers_down<kRoleRegisters>();
+        if (warp == 0 && lane == 0) produce<kTerms, false>(smem, bars, walk);
+        if (warp == 2 && lane == 0) produce<kTerms, true>(smem, bars, walk);
+        if (warp == 1 && lane == 0) multiply<kTerms, kRun>(smem, bars, tmem, walk);
         __syncwarp();
     } else {
+        tc::registers_up<kEpiRegisters>();
         epi(smem, bars, tmem, warp, lane);
     }
     tc::tc_fence_before();
@@ -348,55 +379,71 @@ struct LogitArgs {
     const int32_t *labels;
     float scale;
     // forward
-    float2 *partial;  // [2 splits][rows] (maximum, sum)
-    float *target;    // [rows] logit of the label
+    float2 *partial;  // [2 splits][rows] (maximum, sum), logits in units of ln 2
+    float *target;    // [rows] logit of the label, in units of ln 2
     // backward
     const float *lse, *dloss;
     float *column_sums;  // [4 m_tiles][count] or null
 };
 
-// Item i: row tiles in groups of kGroupM, the items of a group by columns
-// first, so that the CTAs of a wave share kGroupM row tiles and few units.
-__device__ __forceinline__ void item_at(const LogitArgs &a, int64_t item, int &m, int &split) {
-    const int64_t group = item / (static_cast<int64_t>(kGroupM) * a.splits);
-    const int64_t rest = item - group * kGroupM * a.splits;
-    const int rows = min(kGroupM, a.m_tiles - static_cast<int>(group) * kGroupM);
-    split = static_cast<int>(rest / rows);
-    m = static_cast<int>(group) * kGroupM + static_cast<int>(rest % rows);
-}
+// The CTA's items, then each item's column tiles.  Items are row tiles in
+// groups of kGroupM, the items of a group by columns first, so that the CTAs
+// of a wave share kGroupM row tiles and few units.  32-bit arithmetic, two
+// divisions an item: the loading and the MMA lane walk between tiles.
+struct LogitWalk {
+    const LogitArgs &a;
+    const CUtensorMap *map_x, *map_w;
+    uint32_t item, items;
+    int m = 0, n = 0, end = 0;
+
+    __device__ __forceinline__ LogitWalk(const LogitArgs &args, const CUtensorMap *x, const CUtensorMap *w)
+        : a(args), map_x(x), map_w(w), item(blockIdx.x), items(static_cast<uint32_t>(args.m_tiles) * args.splits) {}
+    // Column tiles [n, end) of row tile m.
+    __device__ __forceinline__ bool next_item() {
+        if (item >= items) return false;
+        const uint32_t group = item / (kGroupM * static_cast<uint32_t>(a.splits));
+        const uint32_t rest = item - group * kGroupM * a.splits;
+        const uint32_t rows = min(static_cast<uint32_t>(kGroupM), a.m_tiles - group * kGroupM);
+        const uint32_t split = rest / rows;
+        m = static_cast<int>(group * kGroupM + rest - split * rows);
+        n = static_cast<int>(split) * a.span;
+        end = min(n + a.span, a.n_tiles);
+        item += gridDim.x;
+        return true;
+    }
+    __device__ __forceinline__ bool next(Tile &t) {
+        if (n == end && !next_item()) return false;
+        t.a = map_x, t.b = map_w, t.a_mn = t.b_mn = false;
+        t.m0 = m * kTileM;
+        t.n0 = n * a.tile_n;  // map_w covers the launch's units
+        t.n_cols = min(a.tile_n, (a.count - t.n0 + 15) / 16 * 16);
+        t.k0 = 0;
+        t.k1 = a.k_blocks;
+        ++n;
+        return true;
+    }
+};
 
 template <int kTerms, bool kBackward>
 __global__ void __launch_bounds__(kThreads, 1)
     logit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                  const __grid_constant__ CUtensorMap map_g, const LogitArgs a) {
     using S = Shape<kTerms>;
-    const int64_t items = static_cast<int64_t>(a.m_tiles) * a.splits;
-    auto tile = [&](int64_t i, Tile &t) {
-        const int64_t item = blockIdx.x + (i / a.span) * gridDim.x;
-        if (item >= items) return false;
-        int m, split;
-        item_at(a, item, m, split);
-        const int n = split * a.span + static_cast<int>(i % a.span);
-        t.a = &map_x, t.b = &map_w, t.a_mn = t.b_mn = false;
-        t.m0 = m * kTileM;
-        t.a_boxes = a.rows - t.m0 > kBox ? 2 : 1;
-        const int at = n * a.tile_n;
-        t.n0 = at;  // map_w covers the launch's units
-        t.n_cols = min(a.tile_n, (max(a.count - at, 1) + 15) / 16 * 16);
-        t.k0 = 0;
-        t.k1 = n < a.n_tiles ? a.k_blocks : 0;  // the last item of a row may be short
-        return true;
-    };
-    run_roles<kTerms>(tile, [&](uint8_t *smem, const Bars &bars, uint32_t tmem, int warp, int lane) {
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
-        float *bias_slot = reinterpret_cast<float *>(smem + S::kBiasOff) + (warp - 2) * 32;
-        uint8_t *staging = smem + S::kStagingOff + (warp - 2) * 2048;
+    const LogitWalk walk(a, &map_x, &map_w);
+    run_roles<kTerms, kShortRun>(walk, [&](uint8_t *smem, const Bars &bars, uint32_t tmem, int warp, int lane) {
+        const int quarter = warp & 3, ew = warp - kFirstEpi, half = ew >> 2;
+        constexpr int kMax = S::kTileN / 2 / 32;
+        float *bias_slot = reinterpret_cast<float *>(smem + S::kBiasOff) + ew * (S::kTileN / 2);
+        uint8_t *staging = smem + S::kStagingOff + ew * 2048;
         const int half_cols = a.tile_n / 2, chunks = half_cols / 32;
         const uint32_t half_at = (static_cast<uint32_t>(quarter * 32) << 16) + half * half_cols;
-        Columns<kTerms> columns;
-        for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-            int m, split;
-            item_at(a, item, m, split);
+        // logits in units of ln 2, z log2(e): exponentials are powers of two
+        const float2 scale = make_float2(a.scale * kLog2e, a.scale * kLog2e);
+        Columns<kTerms, kShortRun> columns;
+        auto &v = columns.v;
+        LogitWalk own = walk;
+        while (own.next_item()) {
+            const int m = own.m;
             const int64_t row = static_cast<int64_t>(m) * kTileM + quarter * 32 + lane;
             const bool live = row < a.rows;
             int32_t label = live ? a.labels[row] : -1;
@@ -406,86 +453,117 @@ __global__ void __launch_bounds__(kThreads, 1)
             float lse = 0.0f, grad = 0.0f;      // backward
             if constexpr (kBackward) {
                 if (valid) {
-                    lse = a.lse[row];
+                    lse = a.lse[row] * kLog2e;
                     grad = a.dloss[row];
                 }
             }
-            for (int n = split * a.span; n < min((split + 1) * a.span, a.n_tiles); ++n) {
+            for (int n = own.n; n < own.end; ++n) {
                 const int col0 = n * a.tile_n + half * half_cols;  // within the launch's units
-                float bias[Columns<kTerms>::kMax];
+                // bias of the half's columns, and which take no part: units
+                // left out and columns past the last, -inf whatever the product is
+                uint32_t out[kMax];
+                __syncwarp();
 #pragma unroll
-                for (int j = 0; j < Columns<kTerms>::kMax; ++j) {
+                for (int j = 0; j < kMax; ++j) {
                     const int c = col0 + 32 * j + lane;
-                    bias[j] = c >= a.count ? -INFINITY : a.bias ? __ldg(a.bias + a.first + c) : 0.0f;
+                    const float b = c >= a.count ? -INFINITY : a.bias ? __ldg(a.bias + a.first + c) : 0.0f;
+                    bias_slot[32 * j + lane] = b * kLog2e;
+                    out[j] = __ballot_sync(0xFFFFFFFFu, b == -INFINITY);
                 }
-                columns.open(bars, tmem, half_at, chunks, a.k_blocks);
+                __syncwarp();
+                columns.load(bars, tmem, half_at, a.k_blocks);
 #pragma unroll
-                for (int j = 0; j < Columns<kTerms>::kMax; ++j) {
+                for (int j = 0; j < kMax; ++j) {
                     if (j >= chunks) break;
-                    const int col = col0 + 32 * j;
-                    float v[32];
-                    columns.take(tmem, half_at, j, v);
-                    if (a.bias) {
-                        __syncwarp();
-                        bias_slot[lane] = bias[j];
-                        __syncwarp();
+                    const float4 *b4 = reinterpret_cast<const float4 *>(bias_slot + 32 * j);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = fmaf(v[i], a.scale, bias_slot[i]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] *= a.scale;
+                    for (int i = 0; i < 32; i += 4) {
+                        const float4 b = b4[i / 4];
+                        const float2 lo = fma2(make_float2(v[j][i], v[j][i + 1]), scale, make_float2(b.x, b.y));
+                        const float2 hi = fma2(make_float2(v[j][i + 2], v[j][i + 3]), scale, make_float2(b.z, b.w));
+                        v[j][i] = lo.x, v[j][i + 1] = lo.y, v[j][i + 2] = hi.x, v[j][i + 3] = hi.y;
                     }
-                    // units left out and columns past the last: -inf whatever the product is
-                    const uint32_t out = __ballot_sync(0xFFFFFFFFu, bias[j] == -INFINITY);
-                    if (out) {
+                    if (out[j]) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
-                            if (out >> i & 1) v[i] = -INFINITY;
+                            if (out[j] >> i & 1) v[j][i] = -INFINITY;
                     }
-                    const int hit = label - a.first - col;  // the label's column in this chunk
-                    const bool mine = valid && hit >= 0 && hit < 32;
-                    if constexpr (!kBackward) {
-                        if (mine) {
+                }
+                if constexpr (!kBackward) {
+                    const int hit = label - a.first - col0;  // the label's column in the half
+                    if (valid && hit >= 0 && hit < half_cols) {
+#pragma unroll
+                        for (int j = 0; j < kMax; ++j)
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
-                                if (i == hit) a.target[row] = v[i];
+                                if (32 * j + i == hit) a.target[row] = v[j][i];
+                    }
+                    float m8[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) m8[i] = top;
+#pragma unroll
+                    for (int j = 0; j < kMax; ++j) {
+                        if (j >= chunks) break;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2)
+                            m8[i / 2 & 7] = fmaxf(m8[i / 2 & 7], fmaxf(v[j][i], v[j][i + 1]));
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) m8[i] = fmaxf(m8[i], m8[i + 4]);
+                    const float next = fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3]));
+                    const float base = next == -INFINITY ? 0.0f : next;
+                    const float2 minus = make_float2(-base, -base);
+                    float2 s4[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s4[i] = make_float2(0.0f, 0.0f);
+#pragma unroll
+                    for (int j = 0; j < kMax; ++j) {
+                        if (j >= chunks) break;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 d = add2(make_float2(v[j][i], v[j][i + 1]), minus);
+                            s4[i / 2 & 3] = add2(s4[i / 2 & 3], make_float2(exp2_approx(d.x), exp2_approx(d.y)));
                         }
-                        float m8[8];
+                    }
+                    const float2 s = add2(add2(s4[0], s4[1]), add2(s4[2], s4[3]));
+                    sum = fmaf(sum, exp2_approx(top - base), s.x + s.y);
+                    top = next;
+                } else {
+                    const float2 minus = make_float2(-lse, -lse), by = make_float2(grad, grad);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) m8[i] = fmaxf(fmaxf(v[i], v[i + 8]), fmaxf(v[i + 16], v[i + 24]));
+                    for (int j = 0; j < kMax; ++j) {
+                        if (j >= chunks) break;
+                        const int col = col0 + 32 * j;
+                        const int hit = label - a.first - col;  // the label's column in the chunk
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) m8[i] = fmaxf(m8[i], m8[i + 4]);
-                        const float next = fmaxf(top, fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])));
-                        const float base = next == -INFINITY ? 0.0f : next;
-                        float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) s4[i & 3] += exp2_approx((v[i] - base) * kLog2e);
-                        sum = fmaf(sum, exp2_approx((top - base) * kLog2e), (s4[0] + s4[1]) + (s4[2] + s4[3]));
-                        top = next;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = exp2_approx((v[i] - lse) * kLog2e);
-                        if (mine && !(out >> hit & 1)) {
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 d = add2(make_float2(v[j][i], v[j][i + 1]), minus);
+                            v[j][i] = exp2_approx(d.x), v[j][i + 1] = exp2_approx(d.y);
+                        }
+                        if (valid && hit >= 0 && hit < 32) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
-                                if (i == hit) v[i] -= 1.0f;
+                                if (i == hit) v[j][i] -= 1.0f;
                         }
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] *= grad;
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 g = mul2(make_float2(v[j][i], v[j][i + 1]), by);
+                            v[j][i] = g.x, v[j][i + 1] = g.y;
+                        }
                         if (!valid) {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+                            for (int i = 0; i < 32; ++i) v[j][i] = 0.0f;
                         }
-                        if (out) {  // 0, also where lse is -inf
+                        if (out[j]) {  // 0, also where lse is -inf
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
-                                if (out >> i & 1) v[i] = 0.0f;
+                                if (out[j] >> i & 1) v[j][i] = 0.0f;
                         }
                         if (a.column_sums) {
                             // lane i ends with column i's sum over the warp's 32 rows
                             float s[32];
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) s[i] = v[i];
+                            for (int i = 0; i < 32; ++i) s[i] = v[j][i];
 #pragma unroll
                             for (int o = 16; o; o >>= 1) {
                                 const bool upper = lane & o;
@@ -510,12 +588,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
                                     const int i = 8 * c + 2 * e;
-                                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[i], v[i + 1]);
+                                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[j][i], v[j][i + 1]);
                                     w[e] = *reinterpret_cast<const uint32_t *>(&b);
                                     if (p + 1 < kTerms) {
                                         const float2 f = __bfloat1622float2(b);
-                                        v[i] -= f.x;
-                                        v[i + 1] -= f.y;
+                                        v[j][i] -= f.x;
+                                        v[j][i + 1] -= f.y;
                                     }
                                 }
                                 // 64-byte rows, 16-byte units swizzled as SWIZZLE_64B expects
@@ -532,10 +610,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                 }
-                columns.close(bars);
             }
             if constexpr (!kBackward) {
-                if (live) a.partial[(static_cast<int64_t>(split) * 2 + half) * a.rows + row] = make_float2(top, sum);
+                if (live) a.partial[(own.n / a.span * 2 + half) * a.rows + row] = make_float2(top, sum);
             }
         }
         if constexpr (kBackward) {
@@ -556,17 +633,17 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2 *partial, const 
         const float2 p = partial[static_cast<int64_t>(s) * rows + row];
         const float next = fmaxf(top, p.x);
         const float base = next == -INFINITY ? 0.0f : next;
-        sum = sum * exp2_approx((top - base) * kLog2e) + p.y * exp2_approx((p.x - base) * kLog2e);
+        sum = sum * exp2_approx(top - base) + p.y * exp2_approx(p.x - base);
         top = next;
     }
-    const float l = top == -INFINITY && sum == 0.0f ? top : top + logf(sum);
-    lse[row] = l;
+    const float l = top == -INFINITY && sum == 0.0f ? top : top + log2f(sum);
+    lse[row] = l * kLn2;
     const int32_t t = labels[row];
     if (t < 0 || t >= k) {
         loss[row] = 0.0f;
     } else {
         const float z = target[row];
-        loss[row] = z == -INFINITY ? INFINITY : l - z;
+        loss[row] = z == -INFINITY ? INFINITY : (l - z) * kLn2;
     }
 }
 
@@ -578,7 +655,7 @@ struct ProductArgs {
     struct One {
         int32_t m_size, m_tiles;  // rows of the result
         int32_t k_blocks, splits, split_blocks;
-        int64_t items;
+        uint32_t items;
         void *out;            // the result, where a tile has all of its sum
         float *part;          // else f32 [splits][m_size][width]
         bool add;             // to what `part` holds from the pieces before
@@ -590,59 +667,68 @@ struct ProductArgs {
     bool bf16, wide;        // result type; 16-byte stores fit
 };
 
-struct ProductItem {
-    int which, m, n, split;
-};
-__device__ __forceinline__ bool product_at(const ProductArgs &a, int64_t item, ProductItem &p) {
-    p.which = a.first_product;
-    if (item >= a.one[p.which].items) {
-        item -= a.one[p.which].items;
-        p.which ^= 1;
-        if (item >= a.one[p.which].items) return false;
+// The CTA's items: the longer product's first.
+struct ProductWalk {
+    const ProductArgs &a;
+    const CUtensorMap *map_g, *map_gt, *map_w, *map_x;
+    uint32_t item;
+    int which = 0, m = 0, n = 0, split = 0;
+
+    __device__ __forceinline__ ProductWalk(const ProductArgs &args, const CUtensorMap *g, const CUtensorMap *gt,
+                                           const CUtensorMap *w, const CUtensorMap *x)
+        : a(args), map_g(g), map_gt(gt), map_w(w), map_x(x), item(blockIdx.x) {}
+    __device__ __forceinline__ bool next_item() {
+        uint32_t i = item;
+        item += gridDim.x;
+        which = a.first_product;
+        if (i >= a.one[which].items) {
+            i -= a.one[which].items;
+            which ^= 1;
+            if (i >= a.one[which].items) return false;
+        }
+        // columns first, then splits: neighbours share their rows of G
+        const uint32_t rest = i / a.n_tiles;
+        n = static_cast<int>(i - rest * a.n_tiles);
+        split = static_cast<int>(rest / a.one[which].m_tiles);
+        m = static_cast<int>(rest) - split * a.one[which].m_tiles;
+        return true;
     }
-    const auto &o = a.one[p.which];
-    // columns first, then splits: neighbours share their rows of G
-    p.n = static_cast<int>(item % a.n_tiles);
-    const int64_t rest = item / a.n_tiles;
-    p.m = static_cast<int>(rest % o.m_tiles);
-    p.split = static_cast<int>(rest / o.m_tiles);
-    return true;
-}
+    __device__ __forceinline__ bool next(Tile &t) {
+        if (!next_item()) return false;
+        const auto &o = a.one[which];
+        t.a = which == 0 ? map_g : map_gt, t.b = which == 0 ? map_w : map_x;
+        t.a_mn = which == 1, t.b_mn = true;
+        t.m0 = m * kTileM;
+        t.n0 = n * a.tile_n;
+        t.n_cols = min(a.tile_n, (a.width - t.n0 + 15) / 16 * 16);
+        t.k0 = split * o.split_blocks;
+        t.k1 = min(o.k_blocks, t.k0 + o.split_blocks);
+        return true;
+    }
+};
 
 template <int kTerms>
 __global__ void __launch_bounds__(kThreads, 1)
-    product_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_x,
-                   const __grid_constant__ CUtensorMap map_w, const ProductArgs a) {
-    auto tile = [&](int64_t i, Tile &t) {
-        ProductItem p;
-        if (!product_at(a, blockIdx.x + i * gridDim.x, p)) return false;
-        const auto &o = a.one[p.which];
-        t.a = &map_g, t.b = p.which == 0 ? &map_w : &map_x;
-        t.a_mn = p.which == 1, t.b_mn = true;
-        t.m0 = p.m * kTileM;
-        t.a_boxes = o.m_size - t.m0 > kBox ? 2 : 1;
-        t.n0 = p.n * a.tile_n;
-        t.n_cols = min(a.tile_n, (a.width - t.n0 + 15) / 16 * 16);
-        t.k0 = p.split * o.split_blocks;
-        t.k1 = min(o.k_blocks, t.k0 + o.split_blocks);
-        return true;
-    };
-    run_roles<kTerms>(tile, [&](uint8_t *, const Bars &bars, uint32_t tmem, int warp, int lane) {
-        const int quarter = warp & 3, half = (warp - 2) >> 2;
+    product_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_gt,
+                   const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                   const ProductArgs a) {
+    const ProductWalk walk(a, &map_g, &map_gt, &map_w, &map_x);
+    constexpr int kRun = kTerms == 1 ? kOneRun : kShortRun;
+    run_roles<kTerms, kRun>(walk, [&](uint8_t *, const Bars &bars, uint32_t tmem, int warp, int lane) {
+        const int quarter = warp & 3, half = (warp - kFirstEpi) >> 2;
         const int half_cols = a.tile_n / 2, chunks = half_cols / 32;
         const uint32_t half_at = (static_cast<uint32_t>(quarter * 32) << 16) + half * half_cols;
-        Columns<kTerms> columns;
-        ProductItem p;
-        for (int64_t item = blockIdx.x; product_at(a, item, p); item += gridDim.x) {
+        Columns<kTerms, kRun> columns;
+        ProductWalk p = walk;
+        while (p.next_item()) {
             const auto &o = a.one[p.which];
             const int k0 = p.split * o.split_blocks;
-            columns.open(bars, tmem, half_at, chunks, min(o.k_blocks, k0 + o.split_blocks) - k0);
+            columns.load(bars, tmem, half_at, min(o.k_blocks, k0 + o.split_blocks) - k0);
             const int64_t row = static_cast<int64_t>(p.m) * kTileM + quarter * 32 + lane;
 #pragma unroll
-            for (int j = 0; j < Columns<kTerms>::kMax; ++j) {
+            for (int j = 0; j < columns.kMax; ++j) {
                 if (j >= chunks) break;
-                float v[32];
-                columns.take(tmem, half_at, j, v);
+                float(&v)[32] = columns.v[j];
                 const int col = p.n * a.tile_n + half * half_cols + 32 * j;
                 if (row >= o.m_size || col >= a.width) continue;
                 const int64_t at = row * a.width + col;
@@ -691,7 +777,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            columns.close(bars);
         }
     });
 }
@@ -732,7 +817,7 @@ __global__ void __launch_bounds__(256) dbias_kernel(const float *sums, int64_t p
 
 // ---------------------------------------------------------------- operands
 
-// The products' operands: rows of bf16 terms, padded to whole 16-byte units.
+// The products' operands: rows of bf16 terms, padded with zeros to 64 columns.
 // With `clean`, frames without a label and units left out become zero rows:
 // a zero of G times an infinity or a NaN there would reach the gradients.
 struct StageArgs {
@@ -775,7 +860,10 @@ __global__ void __launch_bounds__(256) stage_kernel(StageArgs a) {
             } else if (a.wide) {
                 constexpr int kVec = 16 / sizeof(T);
 #pragma unroll
-                for (int i = 0; i < 8; i += kVec) load_vec<T, kVec>(src + c + i, v + i);
+                for (int i = 0; i < 8; i += kVec) {
+                    if (c < a.width) load_vec<T, kVec>(src + c + i, v + i);
+                    else for (int e = 0; e < kVec; ++e) v[i + e] = 0.0f;
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = c + i < a.width ? to_f32(src[c + i]) : 0.0f;
@@ -812,25 +900,52 @@ EncodeTiled encode_fn() {
     return fn;
 }
 
-// bf16 terms of [rows][pitch], `plane` elements apart, of which `cols`
-// columns count; boxes of 64
-// rows by 64 columns (loads) or 32 by 32 (G's stores).  What lies outside
+// bf16 terms of [rows][pitch], `plane` elements apart; what lies outside
 // reads as zero and is not written.
-CUtensorMap terms_map(const void *base, int64_t cols, int64_t rows, int64_t pitch, int64_t plane, int terms,
-                      bool store = false) {
-    require(reinterpret_cast<uintptr_t>(base) % 16 == 0 && pitch % 8 == 0, "tensor map alignment");
+struct Terms {
+    const void *base;
+    int64_t cols, rows, pitch, plane;
+    int count;
+};
+CUtensorMap encode(const Terms &t, int rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
+                   CUtensorMapSwizzle swizzle) {
+    require(reinterpret_cast<uintptr_t>(t.base) % 16 == 0 && t.pitch % 8 == 0, "tensor map alignment");
     CUtensorMap map;
-    cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows),
-                          static_cast<cuuint64_t>(terms)};
-    cuuint64_t strides[2] = {static_cast<cuuint64_t>(pitch) * 2, static_cast<cuuint64_t>(plane) * 2};
-    const cuuint32_t side = store ? 32 : kBox;
-    cuuint32_t box[3] = {side, side, 1}, estr[3] = {1, 1, 1};
-    const CUresult rc = encode_fn()(
-        &map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
-        CU_TENSOR_MAP_INTERLEAVE_NONE, store ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint32_t steps[4] = {1, 1, 1, 1};
+    const CUresult rc = encode_fn()(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void *>(t.base), dims,
+                                    strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     require(rc == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed");
     return map;
+}
+// Depth along the columns: boxes of 64 columns by `rows` rows.
+CUtensorMap map_k_major(const Terms &t, int rows) {
+    const cuuint64_t pitch = t.pitch * 2, plane = t.plane * 2;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(t.cols), static_cast<cuuint64_t>(t.rows), 1,
+                                static_cast<cuuint64_t>(t.count)};
+    const cuuint64_t strides[3] = {pitch, plane, plane};
+    const cuuint32_t box[4] = {kBlockK, static_cast<cuuint32_t>(rows), 1, 1};
+    return encode(t, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// Depth along the rows: boxes of 64 rows by `cols` columns, 64 of them at a
+// time.  The pitch is a multiple of 64, so the last run stays in its row;
+// columns past the matrix's own reach only results that nobody stores.
+CUtensorMap map_mn_major(const Terms &t, int cols) {
+    require(t.pitch % 64 == 0, "tensor map pitch");
+    const cuuint64_t pitch = t.pitch * 2, plane = t.plane * 2;
+    const cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(t.rows), static_cast<cuuint64_t>((t.cols + 63) / 64),
+                                static_cast<cuuint64_t>(t.count)};
+    const cuuint64_t strides[3] = {pitch, 128, plane};
+    const cuuint32_t box[4] = {64, kBlockK, static_cast<cuuint32_t>(cols / 64), 1};
+    return encode(t, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// G's stores: 32 by 32.
+CUtensorMap map_store(const Terms &t) {
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(t.cols), static_cast<cuuint64_t>(t.rows),
+                                static_cast<cuuint64_t>(t.count)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(t.pitch) * 2, static_cast<cuuint64_t>(t.plane) * 2};
+    const cuuint32_t box[3] = {32, 32, 1};
+    return encode(t, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // ---------------------------------------------------------------- plans
@@ -869,7 +984,7 @@ ForwardPlan plan_forward(int64_t rows, int k, int width, int dtype, int sms) {
         }
     }
     p.splits = static_cast<int>(ceil_div(p.n_tiles, p.span));
-    p.pitch = (width + 7) / 8 * 8;
+    p.pitch = (width + 63) / 64 * 64;
     size_t at = 0;
     auto put = [&](size_t bytes) {
         const size_t here = at;
@@ -901,7 +1016,7 @@ BackwardPlan plan_backward(int64_t rows, int k, int width, int dtype, int sms) {
     const int64_t fit = kPieceBytes / (std::max<int64_t>(rows, 1) * 2 * terms) / 256 * 256;
     p.piece = std::min<int64_t>(k, std::max<int64_t>(256, fit));
     p.m_tiles = ceil_div(rows, kTileM);
-    p.pitch = (width + 7) / 8 * 8;
+    p.pitch = (width + 63) / 64 * 64;
     p.g_pitch = static_cast<int>((p.piece + 63) / 64 * 64);
     p.tile_n = width > 64 ? (terms == 1 && width > 128 ? 256 : 128) : 64;
     const int64_t n_tiles = ceil_div(width, p.tile_n);
@@ -972,13 +1087,13 @@ void forward(const UnitLoss &a, int sms, cudaStream_t stream) {
     auto *xs = reinterpret_cast<__nv_bfloat16 *>(base + p.xs);
     auto *ws = reinterpret_cast<__nv_bfloat16 *>(base + p.ws);
     const void *x = a.x, *w = a.units;
+    int64_t pitch = a.width;
     if (kTerms > 1 || a.width % 8 || !aligned16(x) || !aligned16(w)) {
         stage<T, kTerms>(a, p.pitch, false, xs, ws, sms, stream);
-        x = xs, w = ws;
+        x = xs, w = ws, pitch = p.pitch;
     }
-    const int64_t plane = static_cast<int64_t>(a.k) * p.pitch;
-    const CUtensorMap map_x = terms_map(x, a.width, a.rows, p.pitch, a.rows * p.pitch, kTerms);
-    const CUtensorMap map_w = terms_map(w, a.width, a.k, p.pitch, plane, kTerms);
+    const CUtensorMap map_x = map_k_major({x, a.width, a.rows, pitch, a.rows * pitch, kTerms}, kTileM);
+    const CUtensorMap map_w = map_k_major({w, a.width, a.k, pitch, a.k * pitch, kTerms}, p.tile_n);
     LogitArgs l{};
     l.rows = a.rows, l.first = 0, l.count = a.k, l.k = a.k;
     l.k_blocks = static_cast<int32_t>(ceil_div(a.width, kBlockK));
@@ -1003,15 +1118,15 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
     auto *xs = reinterpret_cast<__nv_bfloat16 *>(base + p.xs);
     auto *ws = reinterpret_cast<__nv_bfloat16 *>(base + p.ws);
     stage<T, kTerms>(a, p.pitch, true, xs, ws, sms, stream);
-    const CUtensorMap map_x = terms_map(xs, a.width, a.rows, p.pitch, a.rows * p.pitch, kTerms);
+    const int64_t pitch = p.pitch, plane = a.k * pitch;
+    const Terms x{xs, a.width, a.rows, pitch, a.rows * pitch, kTerms};
+    const CUtensorMap map_x = map_k_major(x, kTileM), map_xt = map_mn_major(x, p.tile_n);
     allow_smem(logit_kernel<kTerms, true>, Shape<kTerms>::kSmem);
     allow_smem(product_kernel<kTerms>, Shape<kTerms>::kSmem);
-    const int64_t plane = static_cast<int64_t>(a.k) * p.pitch;
     for (int64_t first = 0; first < a.k; first += p.piece) {
         const int64_t count = std::min<int64_t>(p.piece, a.k - first);
-        const CUtensorMap map_g = terms_map(base + p.g, count, a.rows, p.g_pitch, a.rows * p.g_pitch, kTerms);
-        const CUtensorMap map_g_store = terms_map(base + p.g, count, a.rows, p.g_pitch, a.rows * p.g_pitch, kTerms, true);
-        const CUtensorMap map_w = terms_map(ws + first * p.pitch, a.width, count, p.pitch, plane, kTerms);
+        const Terms g{base + p.g, count, a.rows, p.g_pitch, a.rows * p.g_pitch, kTerms};
+        const Terms w{ws + first * pitch, a.width, count, pitch, plane, kTerms};
         LogitArgs l{};
         l.rows = a.rows, l.first = static_cast<int32_t>(first), l.count = static_cast<int32_t>(count), l.k = a.k;
         l.k_blocks = static_cast<int32_t>(ceil_div(a.width, kBlockK));
@@ -1024,7 +1139,8 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
         l.column_sums = a.dbias ? reinterpret_cast<float *>(base + p.sums) : nullptr;
         int64_t grid = std::min<int64_t>(p.m_tiles * l.splits, sms);
         cuda_check(launch_pdl(logit_kernel<kTerms, true>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
-                              Shape<kTerms>::kSmem, stream, map_x, map_w, map_g_store, l));
+                              Shape<kTerms>::kSmem, stream, map_x, map_k_major(w, l.tile_n),
+                              map_store(g), l));
         ProductArgs q{};
         q.width = a.width, q.tile_n = p.tile_n;
         q.n_tiles = static_cast<int32_t>(ceil_div(a.width, p.tile_n));
@@ -1043,7 +1159,7 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
             o.splits = static_cast<int32_t>(std::min<int64_t>(p.splits[i], depth[i]));
             o.split_blocks = static_cast<int32_t>(ceil_div(depth[i], o.splits));
             o.splits = static_cast<int32_t>(ceil_div(depth[i], o.split_blocks));
-            o.items = static_cast<int64_t>(o.m_tiles) * q.n_tiles * o.splits;
+            o.items = static_cast<uint32_t>(o.m_tiles) * q.n_tiles * o.splits;
             o.out = out[i];
             o.part = p.direct[i] ? nullptr : reinterpret_cast<float *>(base + p.part[i]);
             o.add = i == 0 && first > 0;
@@ -1052,7 +1168,8 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
         q.first_product = q.one[0].split_blocks >= q.one[1].split_blocks ? 0 : 1;
         grid = std::min<int64_t>(q.one[0].items + q.one[1].items, sms);
         cuda_check(launch_pdl(product_kernel<kTerms>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
-                              Shape<kTerms>::kSmem, stream, map_g, map_x, map_w, q));
+                              Shape<kTerms>::kSmem, stream, map_k_major(g, kTileM),
+                              map_mn_major(g, kTileM), map_mn_major(w, p.tile_n), map_xt, q));
         auto join = [&](int i) {
             const auto &o = q.one[i];
             const int64_t n = size[i] * a.width;
