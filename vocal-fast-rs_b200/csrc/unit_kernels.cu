@@ -116,10 +116,14 @@ struct Tile {
 // Results that are rounded to bf16 anyway take one run.
 constexpr int kShortRun = 4, kOneRun = 1 << 30;
 
+// A bounded wait of a whole warp, the same answer for every lane.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) {
+    return __all_sync(0xFFFFFFFFu, tc::mbar_wait(bar, parity, kWaitLimitNs));
+}
+
 struct Bars {
     uint64_t *full, *empty, *acc_full, *acc_empty;
     uint32_t *tmem_slot;
-    volatile int *abort_flag;
 };
 
 template <int kTerms>
@@ -131,12 +135,11 @@ __device__ __forceinline__ Bars bars_at(uint8_t *smem) {
     b.acc_full = b.empty + S::kStages;
     b.acc_empty = b.acc_full + 2;
     b.tmem_slot = reinterpret_cast<uint32_t *>(b.acc_empty + 2);
-    b.abort_flag = reinterpret_cast<volatile int *>(b.tmem_slot + 1);
     return b;
 }
 
-// A loading lane: its operand's blocks of every tile through the stages.  The
-// two operands have a lane each: one lane issues a load in some 170 cycles,
+// A loading warp: its operand's blocks of every tile through the stages.  The
+// two operands have a warp each: a lane issues a load in some 170 cycles,
 // and a stage's MMAs take 512.  `walk.next` gives the CTA's next tile, false
 // past the last.
 template <int kTerms, bool kB, class Walk>
@@ -145,26 +148,28 @@ __device__ __forceinline__ void produce(uint8_t *smem, const Bars &bars, Walk wa
     constexpr uint32_t kBytes = kB ? S::kBBytes : S::kABytes;
     const uint32_t bytes = kTerms * (kB ? walk.a.tile_n * kBlockK * 2 : S::kABytes);
     smem += kB ? kTerms * S::kABytes : 0;
+    const bool leader = tc::elect_one();
     int stage = 0;
     uint32_t phase = 0;
     Tile t, after;
-    bool more = walk.next(t);
-    while (more && !*bars.abort_flag) {
+    bool more = walk.next(t), ok = true;
+    while (more && ok) {
         const CUtensorMap *map = kB ? t.b : t.a;
         const bool mn = kB ? t.b_mn : t.a_mn;
         const int32_t r = kB ? t.n0 : t.m0;
         for (int k = t.k0; k < t.k1; ++k) {
-            if (!tc::mbar_wait(&bars.empty[stage], phase ^ 1, kWaitLimitNs)) {
-                *bars.abort_flag = 1;
-                break;
-            }
-            tc::mbar_arrive_expect_tx(&bars.full[stage], bytes);
-            uint8_t *dst = smem + stage * S::kStageBytes;
-            const int32_t kk = k * kBlockK;
+            ok = warp_wait(&bars.empty[stage], phase ^ 1);
+            if (!ok) break;
+            if (leader) {
+                tc::mbar_arrive_expect_tx(&bars.full[stage], bytes);
+                uint8_t *dst = smem + stage * S::kStageBytes;
+                const int32_t kk = k * kBlockK;
 #pragma unroll
-            for (int p = 0; p < kTerms; ++p)
-                tc::tma_load_4d(dst + p * kBytes, map, &bars.full[stage], mn ? 0 : kk, mn ? kk : r, mn ? r / 64 : 0,
-                                p);
+                for (int p = 0; p < kTerms; ++p)
+                    tc::tma_load_4d(dst + p * kBytes, map, &bars.full[stage], mn ? 0 : kk, mn ? kk : r,
+                                    mn ? r / 64 : 0, p);
+            }
+            __syncwarp();
             if (++stage == S::kStages) {
                 stage = 0;
                 phase ^= 1;
@@ -175,7 +180,7 @@ __device__ __forceinline__ void produce(uint8_t *smem, const Bars &bars, Walk wa
     }
     // let every issued copy land before the CTA can exit
     for (int s = 0; s < S::kStages; ++s) {
-        if (!tc::mbar_wait(&bars.empty[stage], phase ^ 1, kWaitLimitNs)) break;
+        if (!warp_wait(&bars.empty[stage], phase ^ 1)) break;
         if (++stage == S::kStages) {
             stage = 0;
             phase ^= 1;
@@ -183,16 +188,18 @@ __device__ __forceinline__ void produce(uint8_t *smem, const Bars &bars, Walk wa
     }
 }
 
-// MMA lane.  Accumulator buffer b of a run: TMEM columns 256 b (the product,
+// MMA warp, one lane of which issues; the others keep the addresses uniform.
+// Accumulator buffer b of a run: TMEM columns 256 b (the product,
 // or hi hi) and 256 b + 128 (the other terms' products).
 template <int kTerms, int kRun, class Walk>
 __device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32_t tmem, Walk walk) {
     using S = Shape<kTerms>;
+    const bool leader = tc::elect_one();
     int stage = 0;
     uint32_t phase = 0, acc_count = 0;
     Tile t, after;
     bool more = walk.next(t);
-    while (more && !*bars.abort_flag) {
+    while (more) {
         const uint32_t idesc = tc::idesc_f16(kTileM, t.n_cols, 1) | (t.a_mn ? tc::kIdescMnA : 0) |
                                (t.b_mn ? tc::kIdescMnB : 0);
         // descriptors of an operand at shared address 0, and their step (in 16 B) per 16 of depth
@@ -202,47 +209,45 @@ __device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32
         for (int k = t.k0; k < t.k1;) {
             const int stop = t.k1 - k > kRun ? k + kRun : t.k1;
             const uint32_t b = acc_count & 1;
-            if (!tc::mbar_wait(&bars.acc_empty[b], ((acc_count >> 1) & 1) ^ 1, kWaitLimitNs)) {
-                *bars.abort_flag = 1;
-                return;
-            }
+            if (!warp_wait(&bars.acc_empty[b], ((acc_count >> 1) & 1) ^ 1)) return;
             tc::tc_fence_after();
             const uint32_t d = tmem + b * 256;
-            uint32_t big = 0, rest = 0;  // whether each accumulator holds a sum
+            uint32_t held = 0;  // whether the accumulators hold a sum
             for (; k < stop; ++k) {
-                if (!tc::mbar_wait(&bars.full[stage], phase, kWaitLimitNs)) {
-                    *bars.abort_flag = 1;
-                    return;
-                }
+                if (!warp_wait(&bars.full[stage], phase)) return;
                 tc::tc_fence_after();
                 const uint32_t sa = tc::smem_u32(smem + stage * S::kStageBytes), sb = sa + kTerms * S::kABytes;
-                auto product = [&](uint32_t acc, int pa, int pb, uint32_t &held) {
+                auto product = [&](uint32_t acc, int pa, int pb, uint32_t add) {
                     const uint64_t da = a_base + ((sa + pa * S::kABytes) >> 4);
                     const uint64_t db = b_base + ((sb + pb * S::kBBytes) >> 4);
 #pragma unroll
                     for (int kk = 0; kk < kBlockK / 16; ++kk) {
-                        tc::mma_f16(acc, da + kk * a_step, db + kk * b_step, idesc, held);
-                        held = 1;
+                        tc::mma_f16(acc, da + kk * a_step, db + kk * b_step, idesc, kk ? 1 : add);
                     }
                 };
-                if constexpr (kTerms == 1) {
-                    product(d, 0, 0, big);
-                } else {
-                    product(d + 128, 0, 2, rest);
-                    product(d + 128, 2, 0, rest);
-                    product(d + 128, 1, 1, rest);
-                    product(d + 128, 0, 1, rest);
-                    product(d + 128, 1, 0, rest);
-                    product(d, 0, 0, big);
+                if (leader) {
+                    if constexpr (kTerms == 1) {
+                        product(d, 0, 0, held);
+                    } else {
+                        product(d + 128, 0, 2, held);
+                        product(d + 128, 2, 0, 1);
+                        product(d + 128, 1, 1, 1);
+                        product(d + 128, 0, 1, 1);
+                        product(d + 128, 1, 0, 1);
+                        product(d, 0, 0, held);
+                    }
+                    tc::mma_commit(&bars.empty[stage]);
                 }
-                tc::mma_commit(&bars.empty[stage]);
+                __syncwarp();
+                held = 1;
                 if (++stage == S::kStages) {
                     stage = 0;
                     phase ^= 1;
                 }
                 if (k == t.k0) more = walk.next(after);  // while the tensor cores work
             }
-            tc::mma_commit(&bars.acc_full[b]);
+            if (leader) tc::mma_commit(&bars.acc_full[b]);
+            __syncwarp();
             ++acc_count;
         }
         t = after;
@@ -286,11 +291,7 @@ struct Columns {
 
 private:
     __device__ __forceinline__ uint32_t wait(const Bars &bars, uint32_t base) {
-        if (!bad && !tc::mbar_wait(&bars.acc_full[acc_count & 1], (acc_count >> 1) & 1, kWaitLimitNs)) {
-            *bars.abort_flag = 1;
-            bad = true;
-        }
-        bad = __any_sync(0xFFFFFFFFu, bad);
+        if (!bad) bad = !warp_wait(&bars.acc_full[acc_count & 1], (acc_count >> 1) & 1);
         tc::tc_fence_after();
         return base + (acc_count & 1) * 256;
     }
@@ -334,7 +335,6 @@ __device__ __forceinline__ void run_roles(const Walk &walk, Epi epi) {
             tc::mbar_init(&bars.acc_full[b], 1);
             tc::mbar_init(&bars.acc_empty[b], kEpiWarps);
         }
-        *bars.abort_flag = 0;
         tc::fence_mbarrier_init();
     }
     if (warp == 1) {
@@ -348,9 +348,9 @@ __device__ __forceinline__ void run_roles(const Walk &walk, Epi epi) {
     grid_dependency_wait();
     if (warp < kFirstEpi) {
         tc::registers_down<kRoleRegisters>();
-        if (warp == 0 && lane == 0) produce<kTerms, false>(smem, bars, walk);
-        if (warp == 2 && lane == 0) produce<kTerms, true>(smem, bars, walk);
-        if (warp == 1 && lane == 0) multiply<kTerms, kRun>(smem, bars, tmem, walk);
+        if (warp == 0) produce<kTerms, false>(smem, bars, walk);
+        if (warp == 2) produce<kTerms, true>(smem, bars, walk);
+        if (warp == 1) multiply<kTerms, kRun>(smem, bars, tmem, walk);
         __syncwarp();
     } else {
         tc::registers_up<kEpiRegisters>();
