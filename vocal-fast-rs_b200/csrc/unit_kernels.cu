@@ -35,12 +35,13 @@ namespace {
 constexpr int kTileM = 128;      // TMEM lanes
 constexpr int kBlockK = 64;      // bf16 elements of one 128-byte swizzled row
 constexpr uint32_t kBoxBytes = 64 * kBlockK * 2;  // 64 rows of 128 B
-constexpr int kEpiWarps = 8;     // two per lane quarter, each on half of a tile's columns
+constexpr int kEpiWarps = 16;    // four per lane quarter, each on a quarter of a tile's columns
+constexpr int kParts = kEpiWarps / 4;
 constexpr int kFirstEpi = 4;     // warps 0 and 2 load A and B, warp 1 issues MMAs, warp 3 only gives up registers
 constexpr int kThreads = 32 * (kFirstEpi + kEpiWarps);
-// 384 threads launch with 168 registers each: 64,512 = 128 x 72 + 256 x 216.
-constexpr int kRoleRegisters = 72, kEpiRegisters = 216;
-static_assert(128 * kRoleRegisters + 32 * kEpiWarps * kEpiRegisters <= 384 * 168, "register split");
+// 640 threads launch with 96 registers each: 61,440 = 128 x 64 + 512 x 104.
+constexpr int kRoleRegisters = 64, kEpiRegisters = 104;
+static_assert(128 * kRoleRegisters + 32 * kEpiWarps * kEpiRegisters <= kThreads * 96, "register split");
 constexpr int kGroupM = 16;      // row tiles that share the units they read
 constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
@@ -92,8 +93,7 @@ struct Shape {
     static constexpr uint32_t kBBytes = kTileN / 64 * kBoxBytes;
     static constexpr uint32_t kStageBytes = kTerms * (kABytes + kBBytes);
     static constexpr uint32_t kStagingOff = kStages * kStageBytes;
-    static constexpr uint32_t kBiasOff = kStagingOff + kEpiWarps * 2048;
-    static constexpr uint32_t kBarOff = kBiasOff + kEpiWarps * kTileN / 2 * 4;
+    static constexpr uint32_t kBarOff = kStagingOff + kEpiWarps * 2048;
     static constexpr size_t kSmem = 1024 + kBarOff + 256;
     static_assert(kSmem <= 232448, "shared memory");
 };
@@ -254,21 +254,21 @@ __device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32
     }
 }
 
-// Epilogue warps: `load` leaves in v this lane's row of the warp's half of
-// the tile, 32 `chunks` columns of it; all NaN once a wait gave up, so that no
-// result of a call that went wrong looks like one.  The accumulator is free
-// again as soon as it is in registers.
+// Epilogue warps: `load` leaves in v this lane's row of the warp's part of
+// the tile, 32 kMax columns.  The accumulator is free again as soon as it is in
+// registers.  Once a wait gave up (`bad`) v is not to be used, and every later
+// result is NaN, so that none of a call that went wrong looks like one.
 template <int kTerms, int kRun>
 struct Columns {
-    static constexpr int kMax = Shape<kTerms>::kTileN / 2 / 32;  // 32-column chunks of a half
+    static constexpr int kMax = Shape<kTerms>::kTileN / kParts / 32;  // 32-column chunks of a part
     float v[kMax][32];
     uint32_t acc_count = 0;
     bool bad = false;
 
     // All kMax chunks are read, those past a narrow tile's too: their columns
     // exist and nobody uses them.
-    __device__ __forceinline__ void load(const Bars &bars, uint32_t tmem, uint32_t half_at, int depth) {
-        uint32_t at = wait(bars, tmem + half_at);
+    __device__ __forceinline__ void load(const Bars &bars, uint32_t base, int depth) {
+        uint32_t at = wait(bars, base);
 #pragma unroll
         for (int j = 0; j < kMax; ++j) tc::tmem_ld32_nowait(at + 32 * j, v[j]);
 #pragma unroll
@@ -276,16 +276,10 @@ struct Columns {
         if constexpr (kTerms > 1) add_from(at + 128);
         release(bars);
         while (kRun != kOneRun && (depth -= kRun) > 0) {
-            at = wait(bars, tmem + half_at);
+            at = wait(bars, base);
             if constexpr (kTerms > 1) add_from(at + 128);
             add_from(at);
             release(bars);
-        }
-        if (bad) {
-#pragma unroll
-            for (int j = 0; j < kMax; ++j)
-#pragma unroll
-                for (int i = 0; i < 32; ++i) v[j][i] = NAN;
         }
     }
 
@@ -303,14 +297,15 @@ private:
     }
     __device__ __forceinline__ void add_from(uint32_t at) {
 #pragma unroll
-        for (int j = 0; j < kMax; ++j) {
-            float u[32];
-            tc::tmem_ld32_nowait(at + 32 * j, u);
-            tc::tmem_wait_ld32(u);
+        for (int j = 0; j < 2 * kMax; ++j) {
+            float u[16];
+            tc::tmem_ld16_nowait(at + 16 * j, u);
+            tc::tmem_wait_ld(u);
+            float *w = v[j / 2] + 16 * (j & 1);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-                const float2 s = add2(make_float2(v[j][i], v[j][i + 1]), make_float2(u[i], u[i + 1]));
-                v[j][i] = s.x, v[j][i + 1] = s.y;
+            for (int i = 0; i < 16; i += 2) {
+                const float2 s = add2(make_float2(w[i], w[i + 1]), make_float2(u[i], u[i + 1]));
+                w[i] = s.x, w[i + 1] = s.y;
             }
         }
     }
@@ -379,7 +374,7 @@ struct LogitArgs {
     const int32_t *labels;
     float scale;
     // forward
-    float2 *partial;  // [2 splits][rows] (maximum, sum), logits in units of ln 2
+    float2 *partial;  // [kParts splits][rows] (maximum, sum), logits in units of ln 2
     float *target;    // [rows] logit of the label, in units of ln 2
     // backward
     const float *lse, *dloss;
@@ -431,12 +426,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     using S = Shape<kTerms>;
     const LogitWalk walk(a, &map_x, &map_w);
     run_roles<kTerms, kShortRun>(walk, [&](uint8_t *smem, const Bars &bars, uint32_t tmem, int warp, int lane) {
-        const int quarter = warp & 3, ew = warp - kFirstEpi, half = ew >> 2;
-        constexpr int kMax = S::kTileN / 2 / 32;
-        float *bias_slot = reinterpret_cast<float *>(smem + S::kBiasOff) + ew * (S::kTileN / 2);
+        const int quarter = warp & 3, ew = warp - kFirstEpi, part = ew >> 2;
+        constexpr int kMax = Columns<kTerms, kShortRun>::kMax;
+        // 2 KB of the warp's own: a tile's bias first, then G on its way out
         uint8_t *staging = smem + S::kStagingOff + ew * 2048;
-        const int half_cols = a.tile_n / 2, chunks = half_cols / 32;
-        const uint32_t half_at = (static_cast<uint32_t>(quarter * 32) << 16) + half * half_cols;
+        float *bias_slot = reinterpret_cast<float *>(staging);
+        // a tile of 64 columns occupies two parts of 32
+        const int part_cols = max(a.tile_n / kParts, 32), chunks = part * part_cols < a.tile_n ? part_cols / 32 : 0;
+        const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * part_cols;
         // logits in units of ln 2, z log2(e): exponentials are powers of two
         const float2 scale = make_float2(a.scale * kLog2e, a.scale * kLog2e);
         Columns<kTerms, kShortRun> columns;
@@ -453,15 +450,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             float lse = 0.0f, grad = 0.0f;      // backward
             if constexpr (kBackward) {
                 if (valid) {
-                    lse = a.lse[row] * kLog2e;
-                    grad = a.dloss[row];
+                    // every unit left out (-inf): p = 0
+                    lse = a.lse[row] == -INFINITY ? 0.0f : a.lse[row] * kLog2e;
+                    grad = columns.bad ? NAN : a.dloss[row];
                 }
             }
             for (int n = own.n; n < own.end; ++n) {
-                const int col0 = n * a.tile_n + half * half_cols;  // within the launch's units
-                // bias of the half's columns, and which take no part: units
-                // left out and columns past the last, -inf whatever the product is
+                const int col0 = n * a.tile_n + part * part_cols;  // within the launch's units
+                // bias of the part's columns, and which take no part: units
+                // left out and columns past the last
                 uint32_t out[kMax];
+                if constexpr (kBackward) tc::bulk_wait_read<0>();
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < kMax; ++j) {
@@ -471,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     out[j] = __ballot_sync(0xFFFFFFFFu, b == -INFINITY);
                 }
                 __syncwarp();
-                columns.load(bars, tmem, half_at, a.k_blocks);
+                columns.load(bars, base, a.k_blocks);
 #pragma unroll
                 for (int j = 0; j < kMax; ++j) {
                     if (j >= chunks) break;
@@ -483,15 +482,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float2 hi = fma2(make_float2(v[j][i + 2], v[j][i + 3]), scale, make_float2(b.z, b.w));
                         v[j][i] = lo.x, v[j][i + 1] = lo.y, v[j][i + 2] = hi.x, v[j][i + 3] = hi.y;
                     }
-                    if (out[j]) {
+                    // -inf whatever the product is (backward: rows of zeros)
+                    if (!kBackward && out[j]) {
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if (out[j] >> i & 1) v[j][i] = -INFINITY;
                     }
                 }
                 if constexpr (!kBackward) {
-                    const int hit = label - a.first - col0;  // the label's column in the half
-                    if (valid && hit >= 0 && hit < half_cols) {
+                    const int hit = label - a.first - col0;  // the label's column in the part
+                    if (valid && hit >= 0 && hit < 32 * chunks) {
 #pragma unroll
                         for (int j = 0; j < kMax; ++j)
 #pragma unroll
@@ -511,8 +511,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) m8[i] = fmaxf(m8[i], m8[i + 4]);
                     const float next = fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3]));
-                    const float base = next == -INFINITY ? 0.0f : next;
-                    const float2 minus = make_float2(-base, -base);
+                    const float from = next == -INFINITY ? 0.0f : next;
+                    const float2 minus = make_float2(-from, -from);
                     float2 s4[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s4[i] = make_float2(0.0f, 0.0f);
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         }
                     }
                     const float2 s = add2(add2(s4[0], s4[1]), add2(s4[2], s4[3]));
-                    sum = fmaf(sum, exp2_approx(top - base), s.x + s.y);
+                    sum = fmaf(sum, exp2_approx(top - from), s.x + s.y);
                     top = next;
                 } else {
                     const float2 minus = make_float2(-lse, -lse), by = make_float2(grad, grad);
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             const float2 d = add2(make_float2(v[j][i], v[j][i + 1]), minus);
                             v[j][i] = exp2_approx(d.x), v[j][i + 1] = exp2_approx(d.y);
                         }
-                        if (valid && hit >= 0 && hit < 32) {
+                        if (valid && hit >= 0 && hit < 32 && !(out[j] >> hit & 1)) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
                                 if (i == hit) v[j][i] -= 1.0f;
@@ -554,27 +554,28 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int i = 0; i < 32; ++i) v[j][i] = 0.0f;
                         }
-                        if (out[j]) {  // 0, also where lse is -inf
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (out[j] >> i & 1) v[j][i] = 0.0f;
-                        }
                         if (a.column_sums) {
-                            // lane i ends with column i's sum over the warp's 32 rows
-                            float s[32];
+                            // sums over the warp's 32 rows, 16 columns at a
+                            // time: lane i ends with column i & 15
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) s[i] = v[j][i];
+                            for (int h = 0; h < 32; h += 16) {
+                                float s[16];
 #pragma unroll
-                            for (int o = 16; o; o >>= 1) {
-                                const bool upper = lane & o;
+                                for (int i = 0; i < 16; ++i) s[i] = v[j][h + i];
 #pragma unroll
-                                for (int i = 0; i < o; ++i) {
-                                    const float keep = upper ? s[i + o] : s[i];
-                                    s[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, upper ? s[i] : s[i + o], o);
+                                for (int o = 8; o; o >>= 1) {
+                                    const bool upper = lane & o;
+#pragma unroll
+                                    for (int i = 0; i < o; ++i) {
+                                        const float keep = upper ? s[i + o] : s[i];
+                                        s[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, upper ? s[i] : s[i + o], o);
+                                    }
                                 }
+                                s[0] += __shfl_xor_sync(0xFFFFFFFFu, s[0], 16);
+                                const int c = col + h + lane;
+                                if (lane < 16 && c < a.count)
+                                    a.column_sums[(static_cast<int64_t>(m) * 4 + quarter) * a.count + c] = s[0];
                             }
-                            if (col + lane < a.count)
-                                a.column_sums[(static_cast<int64_t>(m) * 4 + quarter) * a.count + col + lane] = s[0];
                         }
                         // G in bf16 (f32: three terms): a factor of its own
                         // products, rounded as any operand of theirs
@@ -612,7 +613,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
             if constexpr (!kBackward) {
-                if (live) a.partial[(own.n / a.span * 2 + half) * a.rows + row] = make_float2(top, sum);
+                if (columns.bad) sum = NAN;
+                if (live) a.partial[(own.n / a.span * kParts + part) * a.rows + row] = make_float2(top, sum);
             }
         }
         if constexpr (kBackward) {
@@ -715,26 +717,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     const ProductWalk walk(a, &map_g, &map_gt, &map_w, &map_x);
     constexpr int kRun = kTerms == 1 ? kOneRun : kShortRun;
     run_roles<kTerms, kRun>(walk, [&](uint8_t *, const Bars &bars, uint32_t tmem, int warp, int lane) {
-        const int quarter = warp & 3, half = (warp - kFirstEpi) >> 2;
-        const int half_cols = a.tile_n / 2, chunks = half_cols / 32;
-        const uint32_t half_at = (static_cast<uint32_t>(quarter * 32) << 16) + half * half_cols;
+        const int quarter = warp & 3, part = (warp - kFirstEpi) >> 2;
+        const int part_cols = max(a.tile_n / kParts, 32), chunks = part * part_cols < a.tile_n ? part_cols / 32 : 0;
+        const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * part_cols;
         Columns<kTerms, kRun> columns;
         ProductWalk p = walk;
         while (p.next_item()) {
             const auto &o = a.one[p.which];
             const int k0 = p.split * o.split_blocks;
-            columns.load(bars, tmem, half_at, min(o.k_blocks, k0 + o.split_blocks) - k0);
+            columns.load(bars, base, min(o.k_blocks, k0 + o.split_blocks) - k0);
             const int64_t row = static_cast<int64_t>(p.m) * kTileM + quarter * 32 + lane;
+            const float scale = columns.bad ? NAN : a.scale;
 #pragma unroll
             for (int j = 0; j < columns.kMax; ++j) {
                 if (j >= chunks) break;
                 float(&v)[32] = columns.v[j];
-                const int col = p.n * a.tile_n + half * half_cols + 32 * j;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] *= scale;
+                const int col = p.n * a.tile_n + part * part_cols + 32 * j;
                 if (row >= o.m_size || col >= a.width) continue;
                 const int64_t at = row * a.width + col;
                 if (o.part == nullptr) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] *= a.scale;
                     if (a.bf16) {
                         __nv_bfloat16 *q = static_cast<__nv_bfloat16 *>(o.out) + at;
                         if (a.wide) {
@@ -781,17 +784,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     });
 }
 
-// out[i] = scale * sum over the splits of part[s][i], in split order.
+// out[i] = sum over the splits of part[s][i], in split order.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const float *part, int64_t stride, int splits, int64_t count,
-                                                   float scale, T *out) {
+                                                   T *out) {
     launch_dependents();
     grid_dependency_wait();
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < count;
          i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         float s = 0.0f;
         for (int k = 0; k < splits; ++k) s += part[k * stride + i];
-        out[i] = from_f32<T>(s * scale);
+        out[i] = from_f32<T>(s);
     }
 }
 
@@ -993,7 +996,7 @@ ForwardPlan plan_forward(int64_t rows, int k, int width, int dtype, int sms) {
     };
     p.xs = put(static_cast<size_t>(terms) * rows * p.pitch * 2);
     p.ws = put(static_cast<size_t>(terms) * k * p.pitch * 2);
-    p.partial = put(static_cast<size_t>(2) * p.splits * rows * sizeof(float2));
+    p.partial = put(static_cast<size_t>(kParts) * p.splits * rows * sizeof(float2));
     p.target = put(static_cast<size_t>(rows) * sizeof(float));
     p.bytes = at;
     return p;
@@ -1108,7 +1111,7 @@ void forward(const UnitLoss &a, int sms, cudaStream_t stream) {
                           Shape<kTerms>::kSmem, stream, map_x, map_w, map_x, l));
     cuda_check(launch_pdl(loss_kernel, dim3(static_cast<unsigned>(ceil_div(a.rows, 256))), dim3(256), 0, stream,
                           static_cast<const float2 *>(l.partial), static_cast<const float *>(l.target), a.labels,
-                          a.rows, 2 * p.splits, static_cast<int>(a.k), a.loss, a.lse));
+                          a.rows, kParts * p.splits, static_cast<int>(a.k), a.loss, a.lse));
 }
 
 template <typename T, int kTerms>
@@ -1176,7 +1179,7 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
             const int64_t blocks = std::min<int64_t>(ceil_div(n, 256), 16 * sms);
             const int splits = i == 0 ? p.splits[0] : o.splits;
             cuda_check(launch_pdl(join_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
-                                  static_cast<const float *>(o.part), o.part_stride, splits, n, a.scale,
+                                  static_cast<const float *>(o.part), o.part_stride, splits, n,
                                   static_cast<T *>(o.out)));
         };
         if (!p.direct[1]) join(1);
