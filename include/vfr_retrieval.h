@@ -420,8 +420,8 @@ VFR_API int vfr_retrieval_blend_sharded(VfrShardedIndex *index, const float *que
  *
  * Matrices are row-major and contiguous, [rows][width] with width in
  * 1..4096, of the element type `dtype`; pointers are memory of one device,
- * on which the call runs whatever the current device, and outputs must not
- * overlap inputs.  The calls are asynchronous on `stream` (stream->stream
+ * on which the call runs whatever the current device (the first one is
+ * checked), and outputs must not overlap inputs.  The calls are asynchronous on `stream` (stream->stream
  * may be the default stream), allocate nothing, can be captured into CUDA
  * graphs, and give the same bits every time.  A workspace is read and
  * written until the call's work on the stream is done; calls that may run at

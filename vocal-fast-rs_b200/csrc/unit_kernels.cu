@@ -624,20 +624,30 @@ __global__ void __launch_bounds__(kThreads, 1)
     });
 }
 
-// Joins the slots of each row.
+// Joins the slots of each row: 32 rows a CTA, a warp for every eighth slot.
 __global__ void __launch_bounds__(256) loss_kernel(const float2 *partial, const float *target, const int32_t *labels,
                                                    int64_t rows, int slots, int k, float *loss, float *lse) {
+    __shared__ float2 joined[8][32];
+    launch_dependents();
     grid_dependency_wait();
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (row >= rows) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float top = -INFINITY, sum = 0.0f;
-    for (int s = 0; s < slots; ++s) {
-        const float2 p = partial[static_cast<int64_t>(s) * rows + row];
+    auto join = [&](float2 p) {
         const float next = fmaxf(top, p.x);
-        const float base = next == -INFINITY ? 0.0f : next;
-        sum = sum * exp2_approx(top - base) + p.y * exp2_approx(p.x - base);
+        const float from = next == -INFINITY ? 0.0f : next;
+        sum = sum * exp2_approx(top - from) + p.y * exp2_approx(p.x - from);
         top = next;
+    };
+    if (row < rows) {
+#pragma unroll 4
+        for (int s = warp; s < slots; s += 8) join(partial[s * rows + row]);
     }
+    joined[warp][lane] = make_float2(top, sum);
+    __syncthreads();
+    if (warp != 0 || row >= rows) return;
+#pragma unroll
+    for (int w = 1; w < 8; ++w) join(joined[w][lane]);
     const float l = top == -INFINITY && sum == 0.0f ? top : top + log2f(sum);
     lse[row] = l * kLn2;
     const int32_t t = labels[row];
@@ -798,24 +808,25 @@ __global__ void __launch_bounds__(256) join_kernel(const float *part, int64_t st
     }
 }
 
-// dbias from the row tiles' column sums, in order: 32 columns a CTA, 8 warps over the rows.
-__global__ void __launch_bounds__(256) dbias_kernel(const float *sums, int64_t parts, int32_t count, float *out) {
-    __shared__ float slots[8][32];
+// dbias from the row tiles' column sums, in order: 32 columns a CTA, 32 warps over the rows.
+__global__ void __launch_bounds__(1024) dbias_kernel(const float *sums, int64_t parts, int32_t count, float *out) {
+    __shared__ float slots[32][33];
     launch_dependents();
     grid_dependency_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int col = blockIdx.x * 32 + lane;
     float s = 0.0f;
-    if (col < count)
-        for (int64_t p = warp; p < parts; p += 8) s += sums[p * count + col];
+    if (col < count) {
+#pragma unroll 8
+        for (int64_t p = warp; p < parts; p += 32) s += sums[p * count + col];
+    }
     slots[warp][lane] = s;
     __syncthreads();
-    if (warp == 0 && col < count) {
-        s = 0.0f;
+    s = slots[lane][warp];  // column `warp` of the CTA, part `lane`
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += slots[i][lane];
-        out[col] = s;
-    }
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    const int c = blockIdx.x * 32 + warp;
+    if (lane == 0 && c < count) out[c] = s;
 }
 
 // ---------------------------------------------------------------- operands
@@ -1011,7 +1022,7 @@ struct BackwardPlan {
     size_t xs, ws, g, sums, part[2], bytes;
 };
 // Bytes of G in the workspace, unless 256 units of every frame take more.
-constexpr int64_t kPieceBytes = int64_t(256) << 20;
+constexpr int64_t kPieceBytes = int64_t(1) << 30;
 
 BackwardPlan plan_backward(int64_t rows, int k, int width, int dtype, int sms) {
     const int terms = terms_of(dtype);
@@ -1067,9 +1078,24 @@ BackwardPlan plan_backward(int64_t rows, int k, int width, int dtype, int sms) {
     return p;
 }
 
-template <class K>
-void allow_smem(K kernel, size_t bytes) {
-    cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+// Lets every kernel of this file use its shared memory, once per device.
+void allow_smem() {
+    static std::mutex lock;
+    static uint64_t done = 0;
+    int device = 0;
+    cuda_check(cudaGetDevice(&device));
+    std::lock_guard<std::mutex> held(lock);
+    if (device < 64 && (done >> device & 1)) return;
+    auto allow = [](auto kernel, size_t bytes) {
+        cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+    };
+    allow(logit_kernel<1, false>, Shape<1>::kSmem);
+    allow(logit_kernel<1, true>, Shape<1>::kSmem);
+    allow(product_kernel<1>, Shape<1>::kSmem);
+    allow(logit_kernel<3, false>, Shape<3>::kSmem);
+    allow(logit_kernel<3, true>, Shape<3>::kSmem);
+    allow(product_kernel<3>, Shape<3>::kSmem);
+    if (device < 64) done |= uint64_t(1) << device;
 }
 
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -1105,11 +1131,11 @@ void forward(const UnitLoss &a, int sms, cudaStream_t stream) {
     l.bias = a.bias, l.labels = a.labels, l.scale = a.scale;
     l.partial = reinterpret_cast<float2 *>(base + p.partial);
     l.target = reinterpret_cast<float *>(base + p.target);
-    allow_smem(logit_kernel<kTerms, false>, Shape<kTerms>::kSmem);
+    allow_smem();
     const int64_t grid = std::min<int64_t>(p.m_tiles * p.splits, sms);
     cuda_check(launch_pdl(logit_kernel<kTerms, false>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
                           Shape<kTerms>::kSmem, stream, map_x, map_w, map_x, l));
-    cuda_check(launch_pdl(loss_kernel, dim3(static_cast<unsigned>(ceil_div(a.rows, 256))), dim3(256), 0, stream,
+    cuda_check(launch_pdl(loss_kernel, dim3(static_cast<unsigned>(ceil_div(a.rows, 32))), dim3(256), 0, stream,
                           static_cast<const float2 *>(l.partial), static_cast<const float *>(l.target), a.labels,
                           a.rows, kParts * p.splits, static_cast<int>(a.k), a.loss, a.lse));
 }
@@ -1124,8 +1150,7 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
     const int64_t pitch = p.pitch, plane = a.k * pitch;
     const Terms x{xs, a.width, a.rows, pitch, a.rows * pitch, kTerms};
     const CUtensorMap map_x = map_k_major(x, kTileM), map_xt = map_mn_major(x, p.tile_n);
-    allow_smem(logit_kernel<kTerms, true>, Shape<kTerms>::kSmem);
-    allow_smem(product_kernel<kTerms>, Shape<kTerms>::kSmem);
+    allow_smem();
     for (int64_t first = 0; first < a.k; first += p.piece) {
         const int64_t count = std::min<int64_t>(p.piece, a.k - first);
         const Terms g{base + p.g, count, a.rows, p.g_pitch, a.rows * p.g_pitch, kTerms};
@@ -1185,7 +1210,7 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
         if (!p.direct[1]) join(1);
         if (!p.direct[0] && first + count == a.k) join(0);
         if (a.dbias)
-            cuda_check(launch_pdl(dbias_kernel, dim3(static_cast<unsigned>(ceil_div(count, 32))), dim3(256), 0,
+            cuda_check(launch_pdl(dbias_kernel, dim3(static_cast<unsigned>(ceil_div(count, 32))), dim3(1024), 0,
                                   stream, static_cast<const float *>(l.column_sums), 4 * p.m_tiles,
                                   static_cast<int32_t>(count), a.dbias + first));
     }

@@ -12,20 +12,14 @@ namespace vfr {
 namespace {
 
 
-// The device of `first` (a required pointer); every pointer given must be
-// device or managed memory of that device, as a kernel would fault on others.
-int pointer_device(const void *first, std::initializer_list<const void *> others) {
-    auto device_of = [](const void *p) {
-        cudaPointerAttributes at{};
-        cuda_check(cudaPointerGetAttributes(&at, p));
-        require(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged,
-                "unit operator arguments must be device memory");
-        return at.device;
-    };
-    const int device = device_of(first);
-    for (const void *p : others)
-        if (p) require(device_of(p) == device, "unit operator arguments live on different devices");
-    return device;
+// The device `p` lives on.  Kernels would fault on host memory, so it is
+// refused; the other arguments are the caller's to keep on the same device.
+int pointer_device(const void *p) {
+    cudaPointerAttributes at{};
+    cuda_check(cudaPointerGetAttributes(&at, p));
+    require(at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged,
+            "unit operator arguments must be device memory");
+    return at.device;
 }
 
 int sm_count(int device) {
@@ -82,7 +76,7 @@ extern "C" int vfr_layer_norm(const void *x, const float *gamma, const float *be
         require(x && y && mean && rstd, "null layer norm binding");
         require(vfr::aligned_to(vfr::dtype_bytes(dtype), {x, y}) && vfr::aligned_to(4, {gamma, beta, mean, rstd}),
                 "misaligned layer norm binding");
-        vfr::DeviceGuard guard(vfr::pointer_device(x, {gamma, beta, y, mean, rstd, packed, exponents}));
+        vfr::DeviceGuard guard(vfr::pointer_device(x));
         vfr::launch_layer_norm({x, gamma, beta, rows, width, dtype, eps, y, mean, rstd, packed, exponents}, s);
         cuda_check(cudaGetLastError());
     });
@@ -112,9 +106,7 @@ extern "C" int vfr_layer_norm_backward(const void *dy, const void *x, const uint
         require(vfr::aligned_to(vfr::dtype_bytes(dtype), {dy, x, dx}) &&
                     vfr::aligned_to(4, {gamma, mean, rstd, dgamma, dbeta}) && vfr::aligned_to(16, {workspace}),
                 "misaligned layer norm binding");
-        vfr::DeviceGuard guard(vfr::pointer_device(
-            rows > 0 ? dy : params && dgamma ? dgamma : dbeta,
-            {x, packed, exponents, mean, rstd, gamma, dx, dgamma, dbeta, workspace}));
+        vfr::DeviceGuard guard(vfr::pointer_device(rows > 0 ? dy : dgamma ? dgamma : dbeta));
         const int sms = vfr::current_sms();
         if (params && rows > 0)
             require(workspace && workspace_bytes >= vfr::norm_backward_workspace(rows, width, sms),
@@ -134,7 +126,7 @@ extern "C" int vfr_checkpoint_pack(const void *x, int64_t rows, int32_t width, i
         if (rows == 0) return;
         require(x && packed && exponents, "null checkpoint binding");
         require(vfr::aligned_to(vfr::dtype_bytes(dtype), {x}), "misaligned checkpoint binding");
-        vfr::DeviceGuard guard(vfr::pointer_device(x, {packed, exponents}));
+        vfr::DeviceGuard guard(vfr::pointer_device(x));
         vfr::launch_checkpoint_pack(x, rows, width, dtype, packed, exponents, s);
         cuda_check(cudaGetLastError());
     });
@@ -148,7 +140,7 @@ extern "C" int vfr_checkpoint_unpack(const uint8_t *packed, const uint8_t *expon
         if (rows == 0) return;
         require(x && packed && exponents, "null checkpoint binding");
         require(vfr::aligned_to(vfr::dtype_bytes(dtype), {x}), "misaligned checkpoint binding");
-        vfr::DeviceGuard guard(vfr::pointer_device(x, {packed, exponents}));
+        vfr::DeviceGuard guard(vfr::pointer_device(x));
         vfr::launch_checkpoint_unpack(packed, exponents, rows, width, dtype, x, s);
         cuda_check(cudaGetLastError());
     });
@@ -175,7 +167,7 @@ extern "C" int vfr_unit_loss(const void *x, const void *units, const float *bias
         require(vfr::aligned_to(vfr::dtype_bytes(dtype), {x, units}) &&
                     vfr::aligned_to(4, {bias, labels, loss, lse}) && vfr::aligned_to(256, {workspace}),
                 "misaligned unit loss binding");
-        vfr::DeviceGuard guard(vfr::pointer_device(x, {units, bias, labels, loss, lse, workspace}));
+        vfr::DeviceGuard guard(vfr::pointer_device(x));
         const int sms = vfr::current_sms();
         const size_t need = vfr::unit_loss_workspace(rows, k, width, dtype, false, sms);
         require(need == 0 || (workspace && workspace_bytes >= need), "unit loss workspace is too small");
@@ -200,8 +192,7 @@ extern "C" int vfr_unit_loss_backward(const void *x, const void *units, const fl
         require(vfr::aligned_to(vfr::dtype_bytes(dtype), {x, units, dx, dunits}) &&
                     vfr::aligned_to(4, {bias, labels, lse, dloss, dbias}) && vfr::aligned_to(256, {workspace}),
                 "misaligned unit loss binding");
-        vfr::DeviceGuard guard(
-            vfr::pointer_device(units, {x, bias, labels, lse, dloss, dx, dunits, dbias, workspace}));
+        vfr::DeviceGuard guard(vfr::pointer_device(units));
         const int sms = vfr::current_sms();
         if (rows == 0) {
             cuda_check(cudaMemsetAsync(dunits, 0, static_cast<size_t>(k) * width * vfr::dtype_bytes(dtype), s));
