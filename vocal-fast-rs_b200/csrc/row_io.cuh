@@ -22,7 +22,15 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 
-// kVec consecutive elements; kVec * sizeof(T) bytes, aligned to that size.
+// kVec consecutive elements as loaded: kVec * sizeof(T) bytes, aligned to that size.
+template <typename T, int kVec>
+struct alignas(sizeof(T) * kVec) RawVec {
+    T e[kVec];
+    __device__ __forceinline__ void values(float *v) const {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) v[i] = to_f32(e[i]);
+    }
+};
 template <typename T, int kVec>
 __device__ __forceinline__ void load_vec(const T *p, float *v) {
     if constexpr (kVec == 1) {
@@ -34,6 +42,19 @@ __device__ __forceinline__ void load_vec(const T *p, float *v) {
         const Pack q = *reinterpret_cast<const Pack *>(p);
 #pragma unroll
         for (int i = 0; i < kVec; ++i) v[i] = to_f32(q.e[i]);
+    }
+}
+// kVec f32 parameters, 16-byte aligned where kVec > 1.
+template <int kVec>
+__device__ __forceinline__ void load_params(const float *p, float *v) {
+    if constexpr (kVec == 1) {
+        v[0] = __ldg(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kVec; i += 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4 *>(p + i));
+            v[i] = f.x, v[i + 1] = f.y, v[i + 2] = f.z, v[i + 3] = f.w;
+        }
     }
 }
 template <typename T, int kVec>
@@ -56,15 +77,10 @@ __device__ __forceinline__ void store_vec(T *p, const float *v) {
 // to at most 448, e4m3's largest value.  A power of two costs no precision in
 // a floating format, x 2^-s is exact wherever e4m3 can hold it, and every
 // host and device gets the same bytes.  Stored as the byte s + 127.
-// `top` holds the largest magnitude's f32 bits (0 for an all-zero block).
+// `top` holds the largest finite magnitude's f32 bits (0 for an all-zero block).
 __device__ __forceinline__ uint32_t checkpoint_exponent(uint32_t top) {
     const int e = static_cast<int>(top >> 23) - 8 + ((top & 0x7FFFFFu) > 0x600000u);
     return e > 0 ? e : 0;
-}
-// The magnitude bits of v for the block maximum; infinities and NaN take no part.
-__device__ __forceinline__ uint32_t checkpoint_magnitude(float v) {
-    const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
-    return b < 0x7F800000u ? b : 0u;
 }
 // 2^-s for the byte s + 127 <= 247 (2^-120 .. 2^127, all normal).
 __device__ __forceinline__ float checkpoint_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
@@ -73,24 +89,22 @@ __device__ __forceinline__ float checkpoint_scale(uint32_t byte) {
     return byte ? __uint_as_float(byte << 23) : __uint_as_float(0x400000u);
 }
 // Two values already multiplied by 2^-s to e4m3 bytes (first in the low
-// byte), to nearest even; infinities become NaN, as the format has none.
+// byte), to nearest even; NaN becomes the format's NaN, infinities its
+// largest value.
 __device__ __forceinline__ uint32_t checkpoint_pair(float a, float b) {
-    uint32_t r = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    if (isinf(a)) r = (r & 0xFF00u) | 0x7Fu;
-    if (isinf(b)) r = (r & 0x00FFu) | 0x7F00u;
-    return r;
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
 __device__ __forceinline__ float checkpoint_value(uint8_t q) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw(q, __NV_E4M3)));
 }
 
-// kVec e4m3 bytes (kVec-byte aligned) times 2^s.
+// kVec e4m3 bytes as loaded.
 template <int kVec>
-__device__ __forceinline__ void load_packed(const uint8_t *p, float scale, float *v) {
-    struct alignas(kVec) Pack {
-        uint8_t e[kVec];
-    };
-    const Pack q = *reinterpret_cast<const Pack *>(p);
+struct alignas(kVec) PackedBytes {
+    uint8_t e[kVec];
+};
+template <int kVec>
+__device__ __forceinline__ void unpack_bytes(const PackedBytes<kVec> &q, float scale, float *v) {
     if constexpr (kVec == 1) {
         v[0] = checkpoint_value(q.e[0]) * scale;
     } else {
@@ -106,9 +120,7 @@ __device__ __forceinline__ void load_packed(const uint8_t *p, float scale, float
 }
 template <int kVec>
 __device__ __forceinline__ void store_packed(uint8_t *p, const float *v, float inverse) {
-    struct alignas(kVec) Pack {
-        uint8_t e[kVec];
-    } q;
+    PackedBytes<kVec> q;
     if constexpr (kVec == 1) {
         q.e[0] = static_cast<uint8_t>(checkpoint_pair(v[0] * inverse, 0.0f));
     } else {
@@ -119,7 +131,7 @@ __device__ __forceinline__ void store_packed(uint8_t *p, const float *v, float i
             q.e[i + 1] = static_cast<uint8_t>(r >> 8);
         }
     }
-    *reinterpret_cast<Pack *>(p) = q;
+    *reinterpret_cast<PackedBytes<kVec> *>(p) = q;
 }
 
 }  // namespace vfr

@@ -77,7 +77,8 @@ extern "C" int vfr_layer_norm(const void *x, const float *gamma, const float *be
         require(vfr::aligned_to(vfr::dtype_bytes(dtype), {x, y}) && vfr::aligned_to(4, {gamma, beta, mean, rstd}),
                 "misaligned layer norm binding");
         vfr::DeviceGuard guard(vfr::pointer_device(x));
-        vfr::launch_layer_norm({x, gamma, beta, rows, width, dtype, eps, y, mean, rstd, packed, exponents}, s);
+        vfr::launch_layer_norm({x, gamma, beta, rows, width, dtype, eps, y, mean, rstd, packed, exponents},
+                               vfr::current_sms(), s);
         cuda_check(cudaGetLastError());
     });
 }
@@ -127,7 +128,7 @@ extern "C" int vfr_checkpoint_pack(const void *x, int64_t rows, int32_t width, i
         require(x && packed && exponents, "null checkpoint binding");
         require(vfr::aligned_to(vfr::dtype_bytes(dtype), {x}), "misaligned checkpoint binding");
         vfr::DeviceGuard guard(vfr::pointer_device(x));
-        vfr::launch_checkpoint_pack(x, rows, width, dtype, packed, exponents, s);
+        vfr::launch_checkpoint_pack(x, rows, width, dtype, packed, exponents, vfr::current_sms(), s);
         cuda_check(cudaGetLastError());
     });
 }
@@ -141,7 +142,7 @@ extern "C" int vfr_checkpoint_unpack(const uint8_t *packed, const uint8_t *expon
         require(x && packed && exponents, "null checkpoint binding");
         require(vfr::aligned_to(vfr::dtype_bytes(dtype), {x}), "misaligned checkpoint binding");
         vfr::DeviceGuard guard(vfr::pointer_device(x));
-        vfr::launch_checkpoint_unpack(packed, exponents, rows, width, dtype, x, s);
+        vfr::launch_checkpoint_unpack(packed, exponents, rows, width, dtype, x, vfr::current_sms(), s);
         cuda_check(cudaGetLastError());
     });
 }

@@ -1,5 +1,5 @@
 // Training a content encoder's unit head: layer norm and its gradients, 8-bit
-// activation checkpoints (norm_kernels.cu), and the softmax cross entropy of
+// activation checkpoints (norm_kernels.cu, checkpoint_kernels.cu), and the softmax cross entropy of
 // frames over a codebook of units with its gradients (unit_kernels.cu).
 // Argument checks and workspace sizes are in units.cpp.
 #pragma once
@@ -28,7 +28,7 @@ struct NormForward {
     float *mean, *rstd;
     uint8_t *packed, *exponents;  // both or neither
 };
-void launch_layer_norm(const NormForward &a, cudaStream_t stream);
+void launch_layer_norm(const NormForward &a, int sms, cudaStream_t stream);
 
 struct NormBackward {
     const void *dy;
@@ -45,9 +45,9 @@ size_t norm_backward_workspace(int64_t rows, int width, int sms);
 void launch_layer_norm_backward(const NormBackward &a, int sms, cudaStream_t stream);
 
 void launch_checkpoint_pack(const void *x, int64_t rows, int width, int dtype, uint8_t *packed, uint8_t *exponents,
-                            cudaStream_t stream);
+                            int sms, cudaStream_t stream);
 void launch_checkpoint_unpack(const uint8_t *packed, const uint8_t *exponents, int64_t rows, int width, int dtype,
-                              void *x, cudaStream_t stream);
+                              void *x, int sms, cudaStream_t stream);
 
 struct UnitLoss {
     const void *x;      // [rows][width]
