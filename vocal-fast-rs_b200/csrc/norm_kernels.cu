@@ -15,18 +15,37 @@
 namespace vfr {
 namespace {
 
+// The lane's columns of a parameter vector, `missing` where there is none.
+template <class S>
+__device__ __forceinline__ void load_columns(const float *p, int width, int warp, int lane, float missing, float *v) {
+#pragma unroll
+    for (int c = 0; c < S::kChunks; ++c) {
+        const int col = S::column(c, warp, lane);
+        if (p && col < width) {
+            load_params<S::kVec>(p + col, v + c * S::kVec);
+        } else {
+#pragma unroll
+            for (int i = 0; i < S::kVec; ++i) v[c * S::kVec + i] = missing;
+        }
+    }
+}
+
 template <class S>
 __global__ void __launch_bounds__(kRowThreads, 2) norm_forward_kernel(NormForward a) {
     using T = typename S::T;
     constexpr int kVec = S::kVec;
-    __shared__ float slots[kRowWarps];
+    __shared__ float slots[4 * kRowWarps];
+    int turn = 0;
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % S::kWpr, group = (threadIdx.x >> 5) / S::kWpr;
     const int width = a.width;
     const float inv_width = 1.0f / static_cast<float>(width);
     const int64_t step = static_cast<int64_t>(gridDim.x) * S::kGroups;
     typename S::Raw q[S::kChunks];
+    float gamma[S::kLane], beta[S::kLane];
     launch_dependents();
     grid_dependency_wait();
+    load_columns<S>(a.gamma, width, warp, lane, 1.0f, gamma);
+    load_columns<S>(a.beta, width, warp, lane, 0.0f, beta);
     int64_t base = static_cast<int64_t>(blockIdx.x) * S::kGroups;
     S::load(static_cast<const T *>(a.x) + (base + group) * width, base + group < a.rows ? width : 0, warp, lane, q);
     for (; base < a.rows; base += step) {
@@ -42,7 +61,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_forward_kernel(NormForwar
 #pragma unroll
             for (int i = 0; i < kVec; ++i) sum += v[i];
         }
-        const float mean = row_sum<S::kWpr>(sum, slots, group, warp) * inv_width;
+        const float mean = row_sum<S::kWpr>(sum, slots, turn, group, warp) * inv_width;
         float sq = 0.0f;
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
@@ -56,7 +75,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_forward_kernel(NormForwar
                 }
             }
         }
-        const float rstd = 1.0f / sqrtf(row_sum<S::kWpr>(sq, slots, group, warp) * inv_width + a.eps);
+        const float rstd = 1.0f / sqrtf(row_sum<S::kWpr>(sq, slots, turn, group, warp) * inv_width + a.eps);
         if (limit && warp == 0 && lane == 0) {
             a.mean[row] = mean;
             a.rstd[row] = rstd;
@@ -66,20 +85,11 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_forward_kernel(NormForwar
         for (int c = 0; c < S::kChunks; ++c) {
             const int col = S::column(c, warp, lane);
             if (col < limit) {
-                float v[kVec], w[kVec];
+                float v[kVec];
                 q[c].values(v);
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) v[i] = (v[i] - mean) * rstd;
-                if (a.gamma) {
-                    load_params<kVec>(a.gamma + col, w);
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) v[i] *= w[i];
-                }
-                if (a.beta) {
-                    load_params<kVec>(a.beta + col, w);
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) v[i] += w[i];
-                }
+                for (int i = 0; i < kVec; ++i)
+                    v[i] = fmaf((v[i] - mean) * rstd, gamma[c * kVec + i], beta[c * kVec + i]);
                 store_vec<T, kVec>(y + col, v);
             }
         }
@@ -125,15 +135,15 @@ struct Source<S, true> {
 
 // A group of kWpr warps walks rows group, group + groups, ...; the parameter
 // sums stay in registers until its last row, then join in shared memory, one
-// partial a CTA.  Two CTAs a SM: 16 warps, each with a row (16-bit types: two)
-// of x and dy in flight.
+// partial a CTA.
 template <class S, bool kPacked>
 __global__ void __launch_bounds__(kRowThreads, 2) norm_backward_kernel(NormBackward a) {
     using T = typename S::T;
     constexpr int kVec = S::kVec;
     constexpr bool kAhead = sizeof(T) == 2;
     extern __shared__ float sums[];  // [2][width]
-    __shared__ float slots[kRowWarps];
+    __shared__ float slots[4 * kRowWarps];
+    int turn = 0;
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % S::kWpr, group = (threadIdx.x >> 5) / S::kWpr;
     const int width = a.width;
     const float inv_width = 1.0f / static_cast<float>(width);
@@ -153,6 +163,8 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_backward_kernel(NormBackw
     };
     launch_dependents();
     grid_dependency_wait();
+    float gamma[S::kLane];
+    load_columns<S>(a.gamma, width, warp, lane, 1.0f, gamma);
     int64_t base = static_cast<int64_t>(blockIdx.x) * S::kGroups;
     if (kAhead) fetch(base + group, x, d, mean, rstd);
     for (; base < a.rows; base += step) {
@@ -165,35 +177,33 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_backward_kernel(NormBackw
         for (int c = 0; c < S::kChunks; ++c) {
             const int col = S::column(c, warp, lane);
             if (col < limit) {
-                float v[kVec], g[kVec], w[kVec];
+                float v[kVec], g[kVec];
                 x.values(c, v);
                 d[c].values(g);
-                if (a.gamma) load_params<kVec>(a.gamma + col, w);
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) {
                     v[i] = (v[i] - mean) * rstd;
                     dg[c * kVec + i] += g[i] * v[i];
                     db[c * kVec + i] += g[i];
-                    if (a.gamma) g[i] *= w[i];
+                    g[i] *= gamma[c * kVec + i];
                     sg += g[i];
                     sgn += g[i] * v[i];
                 }
             }
         }
-        sg = row_sum<S::kWpr>(sg, slots, group, warp) * inv_width;
-        sgn = row_sum<S::kWpr>(sgn, slots, group, warp) * inv_width;
+        row_sums<S::kWpr>(sg, sgn, slots, turn, group, warp);
+        sg *= inv_width, sgn *= inv_width;
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
             const int col = S::column(c, warp, lane);
             if (col < limit) {
-                float v[kVec], g[kVec], w[kVec];
+                float v[kVec], g[kVec];
                 x.values(c, v);
                 d[c].values(g);
-                if (a.gamma) load_params<kVec>(a.gamma + col, w);
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) {
                     v[i] = (v[i] - mean) * rstd;
-                    if (a.gamma) g[i] *= w[i];
+                    g[i] *= gamma[c * kVec + i];
                     g[i] = (g[i] - sg - v[i] * sgn) * rstd;
                 }
                 store_vec<T, kVec>(static_cast<T *>(a.dx) + row * width + col, g);

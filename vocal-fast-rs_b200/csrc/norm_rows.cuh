@@ -1,8 +1,8 @@
-// How the norm and checkpoint kernels hold rows: a row belongs to one warp
-// (width <= 1,024) or to four, kLane values a lane in chunks of kVec (16
-// bytes, or single elements where rows or bases fit no 16-byte access), and a
-// group of warps walks the rows with the next row's loads in flight while it
-// works on the present one.
+// How the norm and checkpoint kernels hold rows: a row belongs to a group of
+// one to eight warps, 8 or 16 values a lane in chunks of kVec (16 bytes, or
+// single elements where rows or bases fit no 16-byte access), and the group
+// walks the rows with the next row's loads in flight while it works on the
+// present one.
 #pragma once
 
 #include <algorithm>
@@ -44,21 +44,31 @@ struct RowShape {
     }
 };
 
-// Sum over the warps of a row; `slots` holds kRowWarps floats and is free
-// again when every thread has passed the next call's first barrier.
+// Sums of a and b over the warps of a row.  `slots` holds two sets of
+// 2 kRowWarps floats, used in turn: a warp can be at most one call ahead of
+// the slowest of its group.
 template <int kWpr>
-__device__ __forceinline__ float row_sum(float v, float *slots, int group, int warp) {
+__device__ __forceinline__ void row_sums(float &a, float &b, float *slots, int &turn, int group, int warp) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    if constexpr (kWpr > 1) {
-        __syncthreads();
-        if ((threadIdx.x & 31) == 0) slots[group * kWpr + warp] = v;
-        __syncthreads();
-        v = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kWpr; ++i) v += slots[group * kWpr + i];
+    for (int o = 16; o; o >>= 1) {
+        a += __shfl_xor_sync(0xFFFFFFFFu, a, o);
+        b += __shfl_xor_sync(0xFFFFFFFFu, b, o);
     }
-    return v;
+    if constexpr (kWpr > 1) {
+        float2 *s = reinterpret_cast<float2 *>(slots) + turn * kRowWarps + group * kWpr;
+        if ((threadIdx.x & 31) == 0) s[warp] = make_float2(a, b);
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * kWpr) : "memory");
+        a = b = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kWpr; ++i) a += s[i].x, b += s[i].y;
+        turn ^= 1;
+    }
+}
+template <int kWpr>
+__device__ __forceinline__ float row_sum(float a, float *slots, int &turn, int group, int warp) {
+    float unused = 0.0f;
+    row_sums<kWpr>(a, unused, slots, turn, group, warp);
+    return a;
 }
 
 // The 8-bit checkpoint of the values a warp holds (converged, zeros past the
@@ -120,31 +130,20 @@ inline bool wide_rows(int width, int dtype, std::initializer_list<const void *> 
     return aligned_to(packed, vec);
 }
 
-// Calls f(RowShape) for the element type, the access width and the values a
-// lane holds: registers follow the width, 8 at a time.
+// Calls f(RowShape) for the element type, the access width and the warps a
+// row takes.
+template <typename T, int kVec, class F>
+void with_row_warps(int width, F &&f) {
+    if (width <= 256) f(RowShape<T, kVec, 1, 8>{});
+    else if (width <= 512) f(RowShape<T, kVec, 1, 16>{});
+    else if (width <= 1024) f(RowShape<T, kVec, 2, 16>{});
+    else if (width <= 2048) f(RowShape<T, kVec, 4, 16>{});
+    else f(RowShape<T, kVec, 8, 16>{});
+}
 template <typename T, class F>
 void with_row_shape(bool wide, int width, F &&f) {
-    constexpr int kVec = 16 / sizeof(T);
-    if (width <= 1024) {
-        if (!wide) {
-            if (width <= 256) f(RowShape<T, 1, 1, 8>{});
-            else f(RowShape<T, 1, 1, 32>{});
-        } else if (width <= 256) {
-            f(RowShape<T, kVec, 1, 8>{});
-        } else if (width <= 512) {
-            f(RowShape<T, kVec, 1, 16>{});
-        } else if (width <= 768) {
-            f(RowShape<T, kVec, 1, 24>{});
-        } else {
-            f(RowShape<T, kVec, 1, 32>{});
-        }
-    } else if (!wide) {
-        f(RowShape<T, 1, 4, 32>{});
-    } else if (width <= 2048) {
-        f(RowShape<T, kVec, 4, 16>{});
-    } else {
-        f(RowShape<T, kVec, 4, 32>{});
-    }
+    if (wide) with_row_warps<T, 16 / sizeof(T)>(width, f);
+    else with_row_warps<T, 1>(width, f);
 }
 template <class F>
 void with_rows(int dtype, bool wide, int width, F &&f) {
@@ -152,7 +151,7 @@ void with_rows(int dtype, bool wide, int width, F &&f) {
     else if (dtype == kBF16) with_row_shape<__nv_bfloat16>(wide, width, f);
     else with_row_shape<__half>(wide, width, f);
 }
-inline int row_groups(int width) { return kRowWarps / (width <= 1024 ? 1 : 4); }
+inline int row_groups(int width) { return width <= 512 ? 8 : width <= 1024 ? 4 : width <= 2048 ? 2 : 1; }
 
 // CTAs for `rows` rows: what the rows fill, or `resident` a SM.
 inline unsigned row_grid(int64_t rows, int groups, int sms, int resident) {
