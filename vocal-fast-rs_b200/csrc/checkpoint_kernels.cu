@@ -2,87 +2,123 @@
 // of a row.  Bound by HBM: packing reads the values and writes a byte each,
 // unpacking the reverse.
 #include "norm_rows.cuh"
-#include "pdl.cuh"
-#include "vfr_common.h"
 
 namespace vfr {
 namespace {
 
 template <class S>
-__global__ void __launch_bounds__(kRowThreads, 2) pack_kernel(const typename S::T *x, int64_t rows, int width, uint8_t *packed,
-                                                              uint8_t *exponents) {
+__global__ void __launch_bounds__(kRowThreads, 2)
+    pack_kernel(const typename S::T *x, int64_t rows, int width, uint8_t *packed, uint8_t *exponents, RingPlan plan) {
+    extern __shared__ uint8_t smem[];
+    __shared__ RingBars bars;
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % S::kWpr, group = (threadIdx.x >> 5) / S::kWpr;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * S::kGroups;
-    const int blocks = checkpoint_blocks(width);
+    const int64_t blocks = (rows + S::kGroups - 1) / S::kGroups;
+    RowRing<S::kGroups> ring{plan, &bars, smem, {reinterpret_cast<const uint8_t *>(x), nullptr}, rows};
+    typename S::Raw q[S::kChunks];
     launch_dependents();
-    grid_dependency_wait();
-    int64_t row = static_cast<int64_t>(blockIdx.x) * S::kGroups + group;
-    typename S::Raw q[S::kChunks], next[S::kChunks];
-    S::load(x + row * width, row < rows ? width : 0, warp, lane, q);
-    for (; row < rows; row += step) {
-        S::load(x + (row + step) * width, row + step < rows ? width : 0, warp, lane, next);
-        pack_row<S>(q, width, warp, lane, packed + row * width, exponents + row * blocks);
+    if constexpr (S::kRing) ring.start([] { grid_dependency_wait(); });
+    else grid_dependency_wait();
+    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+        const int64_t row = block * S::kGroups + group;
+        const int limit = row < rows ? width : 0;
+        if constexpr (S::kRing) {
+            ring.open();
+            S::load(reinterpret_cast<const typename S::T *>(ring.row(0, group)), limit, warp, lane, q);
+            ring.close(block);
+        } else {
+            S::load(x + row * width, limit, warp, lane, q);
+        }
+        if (limit)
+            pack_row<S>(
+                [&](int c, float *v) {
+                    q[c].values(v);
+                    if (ring.bad)
 #pragma unroll
-        for (int c = 0; c < S::kChunks; ++c) q[c] = next[c];
+                        for (int i = 0; i < S::kVec; ++i) v[i] = NAN;
+                },
+                width, warp, lane, packed + row * width, exponents + row * checkpoint_blocks(width));
     }
 }
 
 template <class S>
-__global__ void __launch_bounds__(kRowThreads, 2) unpack_kernel(const uint8_t *packed, const uint8_t *exponents,
-                                                                int64_t rows, int width, typename S::T *x) {
+__global__ void __launch_bounds__(kRowThreads, 2)
+    unpack_kernel(const uint8_t *packed, const uint8_t *exponents, int64_t rows, int width, typename S::T *x,
+                  RingPlan plan) {
     constexpr int kVec = S::kVec;
+    extern __shared__ uint8_t smem[];
+    __shared__ RingBars bars;
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % S::kWpr, group = (threadIdx.x >> 5) / S::kWpr;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * S::kGroups;
-    const int blocks = checkpoint_blocks(width);
+    const int64_t blocks = (rows + S::kGroups - 1) / S::kGroups;
+    RowRing<S::kGroups> ring{plan, &bars, smem, {packed, nullptr}, rows};
     launch_dependents();
-    grid_dependency_wait();
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * S::kGroups + group; row < rows; row += step) {
-        const uint8_t *bytes = packed + row * width, *exps = exponents + row * blocks;
+    if constexpr (S::kRing) ring.start([] { grid_dependency_wait(); });
+    else grid_dependency_wait();
+    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+        const int64_t row = block * S::kGroups + group;
+        const int limit = row < rows ? width : 0;
+        const uint8_t *exps = exponents + row * checkpoint_blocks(width);
         PackedBytes<kVec> q[S::kChunks];
         uint8_t e[S::kChunks];
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
             const int col = S::column(c, warp, lane);
-            if (col < width) {
-                q[c] = *reinterpret_cast<const PackedBytes<kVec> *>(bytes + col);
+            if (col < limit) {
                 e[c] = exps[col / kCheckpointBlock];
+                if (!S::kRing) q[c] = *reinterpret_cast<const PackedBytes<kVec> *>(packed + row * width + col);
             }
+        }
+        if constexpr (S::kRing) {
+            ring.open();
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c) {
+                const int col = S::column(c, warp, lane);
+                if (col < limit) q[c] = *reinterpret_cast<const PackedBytes<kVec> *>(ring.row(0, group) + col);
+            }
+            ring.close(block);
         }
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
             const int col = S::column(c, warp, lane);
-            if (col < width) {
+            if (col < limit) {
                 float v[kVec];
-                unpack_bytes<kVec>(q[c], checkpoint_scale(e[c]), v);
+                unpack_bytes<kVec>(q[c], ring.bad ? NAN : checkpoint_scale(e[c]), v);
                 store_vec<typename S::T, kVec>(x + row * width + col, v);
             }
         }
     }
 }
 
-constexpr int kResident = 4;
+// CTAs a SM: with a ring two, whose rings fill its shared memory.
+constexpr int kResident = 2, kLaneResident = 4;
 
 }  // namespace
 
 void launch_checkpoint_pack(const void *x, int64_t rows, int width, int dtype, uint8_t *packed, uint8_t *exponents,
                             int sms, cudaStream_t stream) {
     if (rows == 0) return;
-    const unsigned grid = row_grid(rows, row_groups(width), sms, kResident);
-    with_rows(dtype, wide_rows(width, dtype, {x}, packed), width, [&](auto s) {
+    const size_t row = width * dtype_bytes(dtype);
+    const bool wide = whole_units(row, {x}) && packs_wide(packed, dtype);
+    const int groups = row_groups(width, wide);
+    const RingPlan plan = plan_ring(groups, row, 0);
+    const unsigned grid = row_grid(rows, groups, sms, wide ? kResident : kLaneResident);
+    with_rows(dtype, wide, width, [&](auto s) {
         using S = decltype(s);
-        cuda_check(launch_pdl(pack_kernel<S>, dim3(grid), dim3(kRowThreads), 0, stream,
-                              static_cast<const typename S::T *>(x), rows, width, packed, exponents));
+        launch_rows(pack_kernel<S>, grid, S::kRing ? ring_bytes(plan, groups) : 0, stream,
+                    static_cast<const typename S::T *>(x), rows, width, packed, exponents, plan);
     });
 }
 
 void launch_checkpoint_unpack(const uint8_t *packed, const uint8_t *exponents, int64_t rows, int width, int dtype,
                               void *x, int sms, cudaStream_t stream) {
     if (rows == 0) return;
-    const unsigned grid = row_grid(rows, row_groups(width), sms, kResident);
-    with_rows(dtype, wide_rows(width, dtype, {x}, packed), width, [&](auto s) {
+    const bool wide = whole_units(width, {packed}) && whole_units(width * dtype_bytes(dtype), {x});
+    const int groups = row_groups(width, wide);
+    const RingPlan plan = plan_ring(groups, width, 0);
+    const unsigned grid = row_grid(rows, groups, sms, wide ? kResident : kLaneResident);
+    with_rows(dtype, wide, width, [&](auto s) {
         using S = decltype(s);
-        cuda_check(launch_pdl(unpack_kernel<S>, dim3(grid), dim3(kRowThreads), 0, stream, packed, exponents, rows,
-                              width, static_cast<typename S::T *>(x)));
+        launch_rows(unpack_kernel<S>, grid, S::kRing ? ring_bytes(plan, groups) : 0, stream, packed, exponents, rows,
+                    width, static_cast<typename S::T *>(x), plan);
     });
 }
 

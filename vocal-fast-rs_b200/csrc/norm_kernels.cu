@@ -9,8 +9,6 @@
 // the variance is the centred sum of squares, not a difference of moments.
 // All sums are f32.
 #include "norm_rows.cuh"
-#include "pdl.cuh"
-#include "vfr_common.h"
 
 namespace vfr {
 namespace {
@@ -31,29 +29,36 @@ __device__ __forceinline__ void load_columns(const float *p, int width, int warp
 }
 
 template <class S>
-__global__ void __launch_bounds__(kRowThreads, 2) norm_forward_kernel(NormForward a) {
+__global__ void __launch_bounds__(kRowThreads, 2) norm_forward_kernel(NormForward a, RingPlan plan) {
     using T = typename S::T;
     constexpr int kVec = S::kVec;
+    extern __shared__ uint8_t smem[];
     __shared__ float slots[4 * kRowWarps];
+    __shared__ RingBars bars;
     int turn = 0;
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % S::kWpr, group = (threadIdx.x >> 5) / S::kWpr;
     const int width = a.width;
     const float inv_width = 1.0f / static_cast<float>(width);
-    const int64_t step = static_cast<int64_t>(gridDim.x) * S::kGroups;
+    const int64_t blocks = (a.rows + S::kGroups - 1) / S::kGroups;
+    RowRing<S::kGroups> ring{plan, &bars, smem, {static_cast<const uint8_t *>(a.x), nullptr}, a.rows};
     typename S::Raw q[S::kChunks];
     float gamma[S::kLane], beta[S::kLane];
     launch_dependents();
-    grid_dependency_wait();
+    if constexpr (S::kRing) ring.start([] { grid_dependency_wait(); });
+    else grid_dependency_wait();
     load_columns<S>(a.gamma, width, warp, lane, 1.0f, gamma);
     load_columns<S>(a.beta, width, warp, lane, 0.0f, beta);
-    int64_t base = static_cast<int64_t>(blockIdx.x) * S::kGroups;
-    S::load(static_cast<const T *>(a.x) + (base + group) * width, base + group < a.rows ? width : 0, warp, lane, q);
-    for (; base < a.rows; base += step) {
-        const int64_t row = base + group, after = row + step;
+    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+        const int64_t row = block * S::kGroups + group;
         const int limit = row < a.rows ? width : 0;
-        typename S::Raw next[S::kChunks];
-        S::load(static_cast<const T *>(a.x) + after * width, after < a.rows ? width : 0, warp, lane, next);
-        float sum = 0.0f;
+        if constexpr (S::kRing) {
+            ring.open();
+            S::load(reinterpret_cast<const T *>(ring.row(0, group)), limit, warp, lane, q);
+            ring.close(block);
+        } else {
+            S::load(static_cast<const T *>(a.x) + row * width, limit, warp, lane, q);
+        }
+        float sum = ring.bad ? NAN : 0.0f;
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
             float v[kVec];
@@ -94,15 +99,20 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_forward_kernel(NormForwar
             }
         }
         if (a.packed && limit)
-            pack_row<S>(q, width, warp, lane, a.packed + row * width, a.exponents + row * checkpoint_blocks(width));
+            pack_row<S>(
+                [&](int c, float *v) {
+                    q[c].values(v);
+                    if (ring.bad)
 #pragma unroll
-        for (int c = 0; c < S::kChunks; ++c) q[c] = next[c];
+                        for (int i = 0; i < kVec; ++i) v[i] = NAN;
+                },
+                width, warp, lane, a.packed + row * width, a.exponents + row * checkpoint_blocks(width));
     }
 }
 
-// x of a row in the backward pass: as it is, or its checkpoint.
+// x of a row in a lane's registers, as it is or its checkpoint.
 template <class S, bool kPacked>
-struct Source {
+struct Held {
     typename S::Raw q[S::kChunks];
     __device__ __forceinline__ void load(const NormBackward &a, int64_t row, int limit, int warp, int lane) {
         S::load(static_cast<const typename S::T *>(a.x) + row * a.width, limit, warp, lane, q);
@@ -110,7 +120,7 @@ struct Source {
     __device__ __forceinline__ void values(int c, float *v) const { q[c].values(v); }
 };
 template <class S>
-struct Source<S, true> {
+struct Held<S, true> {
     PackedBytes<S::kVec> q[S::kChunks];
     uint8_t e[S::kChunks];
     __device__ __forceinline__ void load(const NormBackward &a, int64_t row, int limit, int warp, int lane) {
@@ -121,10 +131,6 @@ struct Source<S, true> {
             if (col < limit) {
                 q[c] = *reinterpret_cast<const PackedBytes<S::kVec> *>(bytes + col);
                 e[c] = exps[col / kCheckpointBlock];
-            } else {
-#pragma unroll
-                for (int i = 0; i < S::kVec; ++i) q[c].e[i] = 0;
-                e[c] = 127;
             }
         }
     }
@@ -133,61 +139,84 @@ struct Source<S, true> {
     }
 };
 
-// A group of kWpr warps walks rows group, group + groups, ...; the parameter
-// sums stay in registers until its last row, then join in shared memory, one
-// partial a CTA.
+// A group of kWpr warps walks its rows; the parameter sums stay in registers
+// until the last one, then join in shared memory, one partial a CTA.  With a
+// ring x and dy are read from shared memory twice, so registers hold only
+// the sums and gamma.
 template <class S, bool kPacked>
-__global__ void __launch_bounds__(kRowThreads, 2) norm_backward_kernel(NormBackward a) {
+__global__ void __launch_bounds__(kRowThreads, 2) norm_backward_kernel(NormBackward a, RingPlan plan) {
     using T = typename S::T;
     constexpr int kVec = S::kVec;
-    constexpr bool kAhead = sizeof(T) == 2;
-    extern __shared__ float sums[];  // [2][width]
+    extern __shared__ uint8_t smem[];  // the ring; at the end the sums [2][width]
     __shared__ float slots[4 * kRowWarps];
+    __shared__ RingBars bars;
     int turn = 0;
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % S::kWpr, group = (threadIdx.x >> 5) / S::kWpr;
     const int width = a.width;
     const float inv_width = 1.0f / static_cast<float>(width);
-    const int64_t step = static_cast<int64_t>(gridDim.x) * S::kGroups;
-    float dg[S::kLane], db[S::kLane];
+    const int64_t blocks = (a.rows + S::kGroups - 1) / S::kGroups;
+    const uint8_t *x_base = kPacked ? a.packed : static_cast<const uint8_t *>(a.x);
+    RowRing<S::kGroups> ring{plan, &bars, smem, {static_cast<const uint8_t *>(a.dy), x_base}, a.rows};
+    float dg[S::kLane], db[S::kLane], gamma[S::kLane];
 #pragma unroll
     for (int i = 0; i < S::kLane; ++i) dg[i] = db[i] = 0.0f;
-    Source<S, kPacked> x, x_next;
-    typename S::Raw d[S::kChunks], d_next[S::kChunks];
+    Held<S, kPacked> x;  // without a ring
+    typename S::Raw d[S::kChunks];
     float mean = 0.0f, rstd = 0.0f, mean_next = 0.0f, rstd_next = 0.0f;
-    auto fetch = [&](int64_t row, Source<S, kPacked> &xs, typename S::Raw(&ds)[S::kChunks], float &m, float &r) {
-        const int limit = row < a.rows ? width : 0;
-        S::load(static_cast<const T *>(a.dy) + row * width, limit, warp, lane, ds);
-        xs.load(a, row, limit, warp, lane);
-        m = limit ? a.mean[row] : 0.0f;
-        r = limit ? a.rstd[row] : 0.0f;
+    auto moments = [&](int64_t block, float &m, float &r) {
+        const int64_t row = block * S::kGroups + group;
+        m = row < a.rows ? a.mean[row] : 0.0f;
+        r = row < a.rows ? a.rstd[row] : 0.0f;
     };
     launch_dependents();
-    grid_dependency_wait();
-    float gamma[S::kLane];
+    if constexpr (S::kRing) ring.start([] { grid_dependency_wait(); });
+    else grid_dependency_wait();
     load_columns<S>(a.gamma, width, warp, lane, 1.0f, gamma);
-    int64_t base = static_cast<int64_t>(blockIdx.x) * S::kGroups;
-    if (kAhead) fetch(base + group, x, d, mean, rstd);
-    for (; base < a.rows; base += step) {
-        const int64_t row = base + group;
+    moments(blockIdx.x, mean_next, rstd_next);
+    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+        const int64_t row = block * S::kGroups + group;
         const int limit = row < a.rows ? width : 0;
-        if (kAhead) fetch(row + step, x_next, d_next, mean_next, rstd_next);
-        else fetch(row, x, d, mean, rstd);
+        mean = mean_next, rstd = rstd_next;
+        moments(block + gridDim.x, mean_next, rstd_next);
+        const uint8_t *exps = nullptr;
+        if constexpr (S::kRing) {
+            if constexpr (kPacked) exps = a.exponents + row * checkpoint_blocks(width);
+            ring.open();
+            if (ring.bad) mean = NAN;
+        } else {
+            S::load(static_cast<const T *>(a.dy) + row * width, limit, warp, lane, d);
+            x.load(a, row, limit, warp, lane);
+        }
+        // chunk c: x as n, and dy
+        auto pair = [&](int c, int col, float *n, float *g) {
+            if constexpr (S::kRing) {
+                load_vec<T, kVec>(reinterpret_cast<const T *>(ring.row(0, group)) + col, g);
+                if constexpr (kPacked)
+                    unpack_bytes<kVec>(*reinterpret_cast<const PackedBytes<kVec> *>(ring.row(1, group) + col),
+                                       checkpoint_scale(__ldg(exps + col / kCheckpointBlock)), n);
+                else
+                    load_vec<T, kVec>(reinterpret_cast<const T *>(ring.row(1, group)) + col, n);
+            } else {
+                d[c].values(g);
+                x.values(c, n);
+            }
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) n[i] = (n[i] - mean) * rstd;
+        };
         float sg = 0.0f, sgn = 0.0f;
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
             const int col = S::column(c, warp, lane);
             if (col < limit) {
-                float v[kVec], g[kVec];
-                x.values(c, v);
-                d[c].values(g);
+                float n[kVec], g[kVec];
+                pair(c, col, n, g);
 #pragma unroll
                 for (int i = 0; i < kVec; ++i) {
-                    v[i] = (v[i] - mean) * rstd;
-                    dg[c * kVec + i] += g[i] * v[i];
+                    dg[c * kVec + i] += g[i] * n[i];
                     db[c * kVec + i] += g[i];
                     g[i] *= gamma[c * kVec + i];
                     sg += g[i];
-                    sgn += g[i] * v[i];
+                    sgn += g[i] * n[i];
                 }
             }
         }
@@ -197,27 +226,19 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_backward_kernel(NormBackw
         for (int c = 0; c < S::kChunks; ++c) {
             const int col = S::column(c, warp, lane);
             if (col < limit) {
-                float v[kVec], g[kVec];
-                x.values(c, v);
-                d[c].values(g);
+                float n[kVec], g[kVec];
+                pair(c, col, n, g);
 #pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    v[i] = (v[i] - mean) * rstd;
-                    g[i] *= gamma[c * kVec + i];
-                    g[i] = (g[i] - sg - v[i] * sgn) * rstd;
-                }
+                for (int i = 0; i < kVec; ++i) g[i] = (g[i] * gamma[c * kVec + i] - sg - n[i] * sgn) * rstd;
                 store_vec<T, kVec>(static_cast<T *>(a.dx) + row * width + col, g);
             }
         }
-        if (kAhead) {
-            x = x_next;
-#pragma unroll
-            for (int c = 0; c < S::kChunks; ++c) d[c] = d_next[c];
-            mean = mean_next, rstd = rstd_next;
-        }
+        if constexpr (S::kRing) ring.close(block);
     }
     if (a.partials == nullptr) return;
     // the CTA's groups one after the other, so the sum's order is fixed
+    float *sums = reinterpret_cast<float *>(smem);
+    __syncthreads();
     for (int g = 0; g < S::kGroups; ++g) {
         if (g == group) {
 #pragma unroll
@@ -267,34 +288,45 @@ __global__ void __launch_bounds__(1024) norm_params_kernel(const float *partials
     }
 }
 
-constexpr int kForwardResident = 4, kBackwardResident = 2;
+// CTAs a SM: with a ring two, whose rings fill its shared memory.
+constexpr int kResident = 2, kLaneResident = 4;
 
 }  // namespace
 
 void launch_layer_norm(const NormForward &a, int sms, cudaStream_t stream) {
     if (a.rows == 0) return;
-    const bool wide = wide_rows(a.width, a.dtype, {a.x, a.y, a.gamma, a.beta}, a.packed);
-    const unsigned grid = row_grid(a.rows, row_groups(a.width), sms, kForwardResident);
+    const size_t row = a.width * dtype_bytes(a.dtype);
+    const bool wide = whole_units(row, {a.x, a.y, a.gamma, a.beta}) && packs_wide(a.packed, a.dtype);
+    const int groups = row_groups(a.width, wide);
+    const RingPlan plan = plan_ring(groups, row, 0);
+    const unsigned grid = row_grid(a.rows, groups, sms, wide ? kResident : kLaneResident);
     with_rows(a.dtype, wide, a.width, [&](auto s) {
-        cuda_check(launch_pdl(norm_forward_kernel<decltype(s)>, dim3(grid), dim3(kRowThreads), 0, stream, a));
+        using S = decltype(s);
+        launch_rows(norm_forward_kernel<S>, grid, S::kRing ? ring_bytes(plan, groups) : 0, stream, a, plan);
     });
 }
 
+// Partials follow the larger grid of the two paths.
 size_t norm_backward_workspace(int64_t rows, int width, int sms) {
-    return static_cast<size_t>(row_grid(rows, row_groups(width), sms, kBackwardResident)) * 2 * width * sizeof(float);
+    const unsigned grid = row_grid(rows, row_groups(width, false), sms, kResident);
+    return static_cast<size_t>(grid) * 2 * width * sizeof(float);
 }
 
 void launch_layer_norm_backward(const NormBackward &args, int sms, cudaStream_t stream) {
     NormBackward a = args;
     if (!a.dgamma && !a.dbeta) a.partials = nullptr;
-    const unsigned grid = row_grid(a.rows, row_groups(a.width), sms, kBackwardResident);
+    unsigned grid = 0;
     if (a.rows > 0) {
-        const bool wide = wide_rows(a.width, a.dtype, {a.dy, a.dx, a.x, a.gamma}, a.packed);
-        const size_t smem = a.partials ? 2 * a.width * sizeof(float) : 0;
+        const size_t row = a.width * dtype_bytes(a.dtype), x_row = a.x ? row : a.width;
+        const bool wide = whole_units(row, {a.dy, a.dx, a.gamma}) && whole_units(x_row, {a.x, a.packed});
+        const int groups = row_groups(a.width, wide);
+        const RingPlan plan = plan_ring(groups, row, x_row);
+        const size_t sums = a.partials ? 2 * a.width * sizeof(float) : 0;
+        grid = row_grid(a.rows, groups, sms, kResident);
         with_rows(a.dtype, wide, a.width, [&](auto s) {
             using S = decltype(s);
-            cuda_check(launch_pdl(a.x ? norm_backward_kernel<S, false> : norm_backward_kernel<S, true>, dim3(grid),
-                                  dim3(kRowThreads), smem, stream, a));
+            launch_rows(a.x ? norm_backward_kernel<S, false> : norm_backward_kernel<S, true>, grid,
+                        std::max(sums, S::kRing ? ring_bytes(plan, groups) : 0), stream, a, plan);
         });
     }
     if (a.dgamma || a.dbeta)
