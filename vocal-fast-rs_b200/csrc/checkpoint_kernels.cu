@@ -9,7 +9,7 @@ namespace {
 template <class S>
 __global__ void __launch_bounds__(kRowThreads, 2)
     pack_kernel(const typename S::T *x, int64_t rows, int width, uint8_t *packed, uint8_t *exponents, RingPlan plan) {
-    extern __shared__ uint8_t smem[];
+    extern __shared__ __align__(128) uint8_t smem[];
     __shared__ RingBars bars;
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % S::kWpr, group = (threadIdx.x >> 5) / S::kWpr;
     const int64_t blocks = (rows + S::kGroups - 1) / S::kGroups;
@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     unpack_kernel(const uint8_t *packed, const uint8_t *exponents, int64_t rows, int width, typename S::T *x,
                   RingPlan plan) {
     constexpr int kVec = S::kVec;
-    extern __shared__ uint8_t smem[];
+    extern __shared__ __align__(128) uint8_t smem[];
     __shared__ RingBars bars;
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % S::kWpr, group = (threadIdx.x >> 5) / S::kWpr;
     const int64_t blocks = (rows + S::kGroups - 1) / S::kGroups;

@@ -32,7 +32,7 @@ template <class S>
 __global__ void __launch_bounds__(kRowThreads, 2) norm_forward_kernel(NormForward a, RingPlan plan) {
     using T = typename S::T;
     constexpr int kVec = S::kVec;
-    extern __shared__ uint8_t smem[];
+    extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float slots[4 * kRowWarps];
     __shared__ RingBars bars;
     int turn = 0;
@@ -58,29 +58,25 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_forward_kernel(NormForwar
         } else {
             S::load(static_cast<const T *>(a.x) + row * width, limit, warp, lane, q);
         }
-        float sum = ring.bad ? NAN : 0.0f;
+        float v[S::kLane];
+        float part[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) part[i] = ring.bad ? NAN : 0.0f;
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
-            float v[kVec];
-            q[c].values(v);
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) sum += v[i];
+            q[c].values(v + c * kVec);
+            add_to<kVec>(part, v + c * kVec);
         }
-        const float mean = row_sum<S::kWpr>(sum, slots, turn, group, warp) * inv_width;
-        float sq = 0.0f;
+        const float mean = row_sum<S::kWpr>(sum_of<kVec>(part), slots, turn, group, warp) * inv_width;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) part[i] = 0.0f;
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
-            if (S::column(c, warp, lane) < limit) {
-                float v[kVec];
-                q[c].values(v);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    const float d = v[i] - mean;
-                    sq += d * d;
-                }
-            }
+            add_scalar<kVec>(v + c * kVec, -mean);
+            if (S::column(c, warp, lane) < limit) fma_to<kVec>(part, v + c * kVec, v + c * kVec);
         }
-        const float rstd = 1.0f / sqrtf(row_sum<S::kWpr>(sq, slots, turn, group, warp) * inv_width + a.eps);
+        const float rstd =
+            1.0f / sqrtf(row_sum<S::kWpr>(sum_of<kVec>(part), slots, turn, group, warp) * inv_width + a.eps);
         if (limit && warp == 0 && lane == 0) {
             a.mean[row] = mean;
             a.rstd[row] = rstd;
@@ -90,21 +86,21 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_forward_kernel(NormForwar
         for (int c = 0; c < S::kChunks; ++c) {
             const int col = S::column(c, warp, lane);
             if (col < limit) {
-                float v[kVec];
-                q[c].values(v);
+                float o[kVec];
 #pragma unroll
-                for (int i = 0; i < kVec; ++i)
-                    v[i] = fmaf((v[i] - mean) * rstd, gamma[c * kVec + i], beta[c * kVec + i]);
-                store_vec<T, kVec>(y + col, v);
+                for (int i = 0; i < kVec; ++i) o[i] = beta[c * kVec + i];
+                mul_scalar<kVec>(v + c * kVec, rstd);
+                fma_to<kVec>(o, v + c * kVec, gamma + c * kVec);
+                store_vec<T, kVec>(y + col, o);
             }
         }
         if (a.packed && limit)
             pack_row<S>(
-                [&](int c, float *v) {
-                    q[c].values(v);
+                [&](int c, float *u) {
+                    q[c].values(u);
                     if (ring.bad)
 #pragma unroll
-                        for (int i = 0; i < kVec; ++i) v[i] = NAN;
+                        for (int i = 0; i < kVec; ++i) u[i] = NAN;
                 },
                 width, warp, lane, a.packed + row * width, a.exponents + row * checkpoint_blocks(width));
     }
@@ -147,7 +143,7 @@ template <class S, bool kPacked>
 __global__ void __launch_bounds__(kRowThreads, 2) norm_backward_kernel(NormBackward a, RingPlan plan) {
     using T = typename S::T;
     constexpr int kVec = S::kVec;
-    extern __shared__ uint8_t smem[];  // the ring; at the end the sums [2][width]
+    extern __shared__ __align__(128) uint8_t smem[];  // the ring; at the end the sums [group][2][width]
     __shared__ float slots[4 * kRowWarps];
     __shared__ RingBars bars;
     int turn = 0;
@@ -187,7 +183,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_backward_kernel(NormBackw
             S::load(static_cast<const T *>(a.dy) + row * width, limit, warp, lane, d);
             x.load(a, row, limit, warp, lane);
         }
-        // chunk c: x as n, and dy
+        // chunk c: x less the mean, and dy
         auto pair = [&](int c, int col, float *n, float *g) {
             if constexpr (S::kRing) {
                 load_vec<T, kVec>(reinterpret_cast<const T *>(ring.row(0, group)) + col, g);
@@ -200,64 +196,68 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_backward_kernel(NormBackw
                 d[c].values(g);
                 x.values(c, n);
             }
-#pragma unroll
-            for (int i = 0; i < kVec; ++i) n[i] = (n[i] - mean) * rstd;
+            add_scalar<kVec>(n, -mean);
         };
-        float sg = 0.0f, sgn = 0.0f;
+        float pg[kVec], pgn[kVec];
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) pg[i] = pgn[i] = 0.0f;
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
             const int col = S::column(c, warp, lane);
             if (col < limit) {
                 float n[kVec], g[kVec];
                 pair(c, col, n, g);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) {
-                    dg[c * kVec + i] += g[i] * n[i];
-                    db[c * kVec + i] += g[i];
-                    g[i] *= gamma[c * kVec + i];
-                    sg += g[i];
-                    sgn += g[i] * n[i];
-                }
+                mul_scalar<kVec>(n, rstd);
+                fma_to<kVec>(dg + c * kVec, g, n);
+                add_to<kVec>(db + c * kVec, g);
+                mul_by<kVec>(g, gamma + c * kVec);
+                add_to<kVec>(pg, g);
+                fma_to<kVec>(pgn, g, n);
             }
         }
+        float sg = sum_of<kVec>(pg), sgn = sum_of<kVec>(pgn);
         row_sums<S::kWpr>(sg, sgn, slots, turn, group, warp);
-        sg *= inv_width, sgn *= inv_width;
+        // dx = rstd (g - mean(g) - n mean(g n)), n = (x - mean) rstd
+        const float shift = -sg * inv_width * rstd, slope = -sgn * inv_width * rstd * rstd;
 #pragma unroll
         for (int c = 0; c < S::kChunks; ++c) {
             const int col = S::column(c, warp, lane);
             if (col < limit) {
                 float n[kVec], g[kVec];
                 pair(c, col, n, g);
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) g[i] = (g[i] * gamma[c * kVec + i] - sg - n[i] * sgn) * rstd;
+                mul_by<kVec>(g, gamma + c * kVec);
+                fma_scalars<kVec>(g, rstd, shift);
+                fma_scalar<kVec>(g, n, slope);
                 store_vec<T, kVec>(static_cast<T *>(a.dx) + row * width + col, g);
             }
         }
         if constexpr (S::kRing) ring.close(block);
     }
     if (a.partials == nullptr) return;
-    // the CTA's groups one after the other, so the sum's order is fixed
+    // each group's sums in shared memory, then joined in group order
     float *sums = reinterpret_cast<float *>(smem);
     __syncthreads();
-    for (int g = 0; g < S::kGroups; ++g) {
-        if (g == group) {
 #pragma unroll
-            for (int c = 0; c < S::kChunks; ++c) {
-                const int col = S::column(c, warp, lane);
-                if (col < width) {
-#pragma unroll
-                    for (int i = 0; i < kVec; ++i) {
-                        float *at = sums + col + i;
-                        at[0] = (g ? at[0] : 0.0f) + dg[c * kVec + i];
-                        at[width] = (g ? at[width] : 0.0f) + db[c * kVec + i];
-                    }
-                }
+    for (int c = 0; c < S::kChunks; ++c) {
+        const int col = S::column(c, warp, lane);
+        if (col < width) {
+            float *at = sums + static_cast<int64_t>(group) * 2 * width + col;
+            store_vec<float, kVec == 1 ? 1 : 4>(at, dg + c * kVec);
+            store_vec<float, kVec == 1 ? 1 : 4>(at + width, db + c * kVec);
+            if constexpr (kVec == 8) {
+                store_vec<float, 4>(at + 4, dg + c * kVec + 4);
+                store_vec<float, 4>(at + width + 4, db + c * kVec + 4);
             }
         }
-        __syncthreads();
     }
+    __syncthreads();
     float *out = a.partials + static_cast<int64_t>(blockIdx.x) * 2 * width;
-    for (int i = threadIdx.x; i < 2 * width; i += kRowThreads) out[i] = sums[i];
+    for (int i = threadIdx.x; i < 2 * width; i += kRowThreads) {
+        float s = 0.0f;
+#pragma unroll
+        for (int g = 0; g < S::kGroups; ++g) s += sums[g * 2 * width + i];
+        out[i] = s;
+    }
 }
 
 // dgamma / dbeta from the CTAs' sums, in order (the same result every time):
@@ -321,7 +321,7 @@ void launch_layer_norm_backward(const NormBackward &args, int sms, cudaStream_t 
         const bool wide = whole_units(row, {a.dy, a.dx, a.gamma}) && whole_units(x_row, {a.x, a.packed});
         const int groups = row_groups(a.width, wide);
         const RingPlan plan = plan_ring(groups, row, x_row);
-        const size_t sums = a.partials ? 2 * a.width * sizeof(float) : 0;
+        const size_t sums = a.partials ? groups * 2 * a.width * sizeof(float) : 0;
         grid = row_grid(a.rows, groups, sms, kResident);
         with_rows(a.dtype, wide, a.width, [&](auto s) {
             using S = decltype(s);

@@ -45,8 +45,7 @@ struct RowShape {
             if (col < limit) {
                 q[c] = *reinterpret_cast<const Raw *>(row + col);
             } else {
-#pragma unroll
-                for (int i = 0; i < kVec; ++i) q[c].e[i] = T(0.0f);
+                q[c].clear();
             }
         }
     }
