@@ -516,7 +516,9 @@ def _head(torch, rows, k, width, dtype, seed, masked=0):
 
 UNIT_SHAPES = [(1, 1, 1), (1, 511, 768), (2, 3, 5), (34, 511, 768), (127, 255, 64), (128, 256, 64), (129, 257, 65),
                (140, 504, 256), (300, 1000, 72), (257, 129, 1000), (1000, 33, 8), (5, 2000, 4096), (700, 640, 200),
-               (64, 64, 128), (1, 5000, 96), (3000, 2, 16)]
+               (64, 64, 128), (1, 5000, 96), (3000, 2, 16),
+               # large enough for CTA pairs, with ragged last tiles on every side
+               (9001, 4611, 256), (6200, 7000, 450)]
 
 
 @pytest.mark.gpu
@@ -665,7 +667,7 @@ def test_unit_loss_several_pieces(cuda, dtype):
     from vfr import units as u
 
     torch = cuda
-    rows, k, width = (100_000, 4000, 64)
+    rows, k, width = (150_000, 4000, 64) if dtype == "bf16" else (50_000, 4000, 64)
     x, w, labels, bias, dloss, scale = _head(torch, rows, k, width, dtype, 11, masked=100)
     dloss = dloss / rows
     loss, lse = u.unit_loss(x, w, labels, scale, bias)

@@ -59,18 +59,39 @@ __device__ __forceinline__ float exp2_approx(float v) {
 // kTerms = 1 (bf16): tiles of 256 columns, 4 stages of A 16 KB + B 32 KB.
 // kTerms = 3 (f32): tiles of 128 columns, 2 stages of three A and three B
 // tiles of 16 KB; per accumulator buffer 128 columns of hi hi, 128 of the rest.
-template <int kTerms>
+// kPair (bf16): a cluster of two CTAs on one M = 256, N = 256 MMA.  CTA r
+// holds the tile's rows 128 r .. of A and columns 128 r .. of B at the same
+// offsets as the other, and its TMEM gets its rows of the result: 32 KB a
+// stage and CTA where one CTA alone reads 48 KB, so that L2 keeps up, and
+// five stages.  The even CTA leads: it issues the MMAs, and every load of a
+// stage counts on its barrier.
+template <int kTerms_, bool kPair_>
 struct Shape {
+    static constexpr int kTerms = kTerms_;
+    static constexpr bool kPair = kPair_;
+    static_assert(!kPair || kTerms == 1, "pairs multiply bf16");
+    static constexpr int kCtas = kPair ? 2 : 1;
     static constexpr int kTileN = kTerms == 1 ? 256 : 128;
-    static constexpr int kStages = kTerms == 1 ? 4 : 2;
+    static constexpr int kStages = kPair ? 5 : kTerms == 1 ? 4 : 2;
     static constexpr uint32_t kABytes = 2 * kBoxBytes;
-    static constexpr uint32_t kBBytes = kTileN / 64 * kBoxBytes;
+    static constexpr uint32_t kBBytes = kTileN / kCtas / 64 * kBoxBytes;
     static constexpr uint32_t kStageBytes = kTerms * (kABytes + kBBytes);
+    // G on its way out, per epilogue warp: 32 rows of 32 columns, of a pair 64
+    static constexpr int kStoreCols = kPair ? 64 : 32;
+    static constexpr uint32_t kStagingBytes = 32 * kStoreCols * 2;
     static constexpr uint32_t kStagingOff = kStages * kStageBytes;
-    static constexpr uint32_t kBarOff = kStagingOff + kEpiWarps * 2048;
+    static constexpr uint32_t kBarOff = kStagingOff + kEpiWarps * kStagingBytes;
     static constexpr size_t kSmem = 1024 + kBarOff + 256;
     static_assert(kSmem <= 232448, "shared memory");
 };
+
+// This CTA among those that share its tiles, and the sharing groups.
+template <class S>
+__device__ __forceinline__ uint32_t tile_rank() { return S::kPair ? blockIdx.x & 1 : 0; }
+template <class S>
+__device__ __forceinline__ uint32_t tile_group() { return blockIdx.x / S::kCtas; }
+template <class S>
+__device__ __forceinline__ uint32_t tile_groups() { return gridDim.x / S::kCtas; }
 
 // A tile of a product: rows m0.., columns n0.. (n_cols of them, a multiple of
 // 16), depth blocks [k0, k1).  One load brings a block of an operand's term:
@@ -100,9 +121,8 @@ struct Bars {
     uint32_t *tmem_slot;
 };
 
-template <int kTerms>
+template <class S>
 __device__ __forceinline__ Bars bars_at(uint8_t *smem) {
-    using S = Shape<kTerms>;
     Bars b;
     b.full = reinterpret_cast<uint64_t *>(smem + S::kBarOff);
     b.empty = b.full + S::kStages;
@@ -116,11 +136,13 @@ __device__ __forceinline__ Bars bars_at(uint8_t *smem) {
 // two operands have a warp each: a lane issues a load in some 170 cycles,
 // and a stage's MMAs take 512.  `walk.next` gives the CTA's next tile, false
 // past the last.
-template <int kTerms, bool kB, class Walk>
+template <class S, bool kB, class Walk>
 __device__ __forceinline__ void produce(uint8_t *smem, const Bars &bars, Walk walk) {
-    using S = Shape<kTerms>;
+    constexpr int kTerms = S::kTerms;
     constexpr uint32_t kBytes = kB ? S::kBBytes : S::kABytes;
-    const uint32_t bytes = kTerms * (kB ? walk.a.tile_n * kBlockK * 2 : S::kABytes);
+    // of both CTAs of a pair
+    const uint32_t bytes = kTerms * (kB ? walk.a.tile_n * kBlockK * 2 : S::kCtas * S::kABytes);
+    const uint32_t rank = tile_rank<S>();
     smem += kB ? kTerms * S::kABytes : 0;
     const bool leader = tc::elect_one();
     int stage = 0;
@@ -130,18 +152,23 @@ __device__ __forceinline__ void produce(uint8_t *smem, const Bars &bars, Walk wa
     while (more && ok) {
         const CUtensorMap *map = kB ? t.b : t.a;
         const bool mn = kB ? t.b_mn : t.a_mn;
-        const int32_t r = kB ? t.n0 : t.m0;
+        const int32_t r = kB ? t.n0 + static_cast<int32_t>(rank) * (S::kTileN / 2) : t.m0;
         for (int k = t.k0; k < t.k1; ++k) {
             ok = warp_wait(&bars.empty[stage], phase ^ 1);
             if (!ok) break;
             if (leader) {
-                tc::mbar_arrive_expect_tx(&bars.full[stage], bytes);
+                if (rank == 0) tc::mbar_arrive_expect_tx(&bars.full[stage], bytes);
                 uint8_t *dst = smem + stage * S::kStageBytes;
                 const int32_t kk = k * kBlockK;
+                if constexpr (S::kPair) {
+                    tc::tma_load_4d_pair(dst, map, tc::map_to_rank(&bars.full[stage], 0), mn ? 0 : kk, mn ? kk : r,
+                                         mn ? r / 64 : 0, 0);
+                } else {
 #pragma unroll
-                for (int p = 0; p < kTerms; ++p)
-                    tc::tma_load_4d(dst + p * kBytes, map, &bars.full[stage], mn ? 0 : kk, mn ? kk : r,
-                                    mn ? r / 64 : 0, p);
+                    for (int p = 0; p < kTerms; ++p)
+                        tc::tma_load_4d(dst + p * kBytes, map, &bars.full[stage], mn ? 0 : kk, mn ? kk : r,
+                                        mn ? r / 64 : 0, p);
+                }
             }
             __syncwarp();
             if (++stage == S::kStages) {
@@ -165,16 +192,16 @@ __device__ __forceinline__ void produce(uint8_t *smem, const Bars &bars, Walk wa
 // MMA warp, one lane of which issues; the others keep the addresses uniform.
 // Accumulator buffer b of a run: TMEM columns 256 b (the product,
 // or hi hi) and 256 b + 128 (the other terms' products).
-template <int kTerms, int kRun, class Walk>
+template <class S, int kRun, class Walk>
 __device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32_t tmem, Walk walk) {
-    using S = Shape<kTerms>;
+    constexpr int kTerms = S::kTerms;
     const bool leader = tc::elect_one();
     int stage = 0;
     uint32_t phase = 0, acc_count = 0;
     Tile t, after;
     bool more = walk.next(t);
     while (more) {
-        const uint32_t idesc = tc::idesc_f16(kTileM, t.n_cols, 1) | (t.a_mn ? tc::kIdescMnA : 0) |
+        const uint32_t idesc = tc::idesc_f16(kTileM * S::kCtas, t.n_cols, 1) | (t.a_mn ? tc::kIdescMnA : 0) |
                                (t.b_mn ? tc::kIdescMnB : 0);
         // descriptors of an operand at shared address 0, and their step (in 16 B) per 16 of depth
         const uint64_t a_base = t.a_mn ? tc::smem_desc_sw128_mn(0, kBoxBytes) : tc::smem_desc_sw128(0);
@@ -196,7 +223,9 @@ __device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32
                     const uint64_t db = b_base + ((sb + pb * S::kBBytes) >> 4);
 #pragma unroll
                     for (int kk = 0; kk < kBlockK / 16; ++kk) {
-                        tc::mma_f16(acc, da + kk * a_step, db + kk * b_step, idesc, kk ? 1 : add);
+                        if constexpr (S::kPair)
+                            tc::mma_f16_pair(acc, da + kk * a_step, db + kk * b_step, idesc, kk ? 1 : add);
+                        else tc::mma_f16(acc, da + kk * a_step, db + kk * b_step, idesc, kk ? 1 : add);
                     }
                 };
                 if (leader) {
@@ -210,7 +239,8 @@ __device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32
                         product(d + 128, 1, 0, 1);
                         product(d, 0, 0, held);
                     }
-                    tc::mma_commit(&bars.empty[stage]);
+                    if constexpr (S::kPair) tc::mma_commit_pair(&bars.empty[stage]);
+                    else tc::mma_commit(&bars.empty[stage]);
                 }
                 __syncwarp();
                 held = 1;
@@ -220,7 +250,10 @@ __device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32
                 }
                 if (k == t.k0) more = walk.next(after);  // while the tensor cores work
             }
-            if (leader) tc::mma_commit(&bars.acc_full[b]);
+            if (leader) {
+                if constexpr (S::kPair) tc::mma_commit_pair(&bars.acc_full[b]);
+                else tc::mma_commit(&bars.acc_full[b]);
+            }
             __syncwarp();
             ++acc_count;
         }
@@ -232,9 +265,10 @@ __device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32
 // the tile, 32 kMax columns.  The accumulator is free again as soon as it is in
 // registers.  Once a wait gave up (`bad`) v is not to be used, and every later
 // result is NaN, so that none of a call that went wrong looks like one.
-template <int kTerms, int kRun>
+template <class S, int kRun>
 struct Columns {
-    static constexpr int kMax = Shape<kTerms>::kTileN / kParts / 32;  // 32-column chunks of a part
+    static constexpr int kTerms = S::kTerms;
+    static constexpr int kMax = S::kTileN / kParts / 32;  // 32-column chunks of a part
     float v[kMax][32];
     uint32_t acc_count = 0;
     bool bad = false;
@@ -266,7 +300,10 @@ private:
     __device__ __forceinline__ void release(const Bars &bars) {
         tc::tc_fence_before();
         __syncwarp();
-        if ((threadIdx.x & 31) == 0) tc::mbar_arrive(&bars.acc_empty[acc_count & 1]);
+        if ((threadIdx.x & 31) == 0) {
+            if constexpr (S::kPair) tc::mbar_arrive_cluster(tc::map_to_rank(&bars.acc_empty[acc_count & 1], 0));
+            else tc::mbar_arrive(&bars.acc_empty[acc_count & 1]);
+        }
         ++acc_count;
     }
     __device__ __forceinline__ void add_from(uint32_t at) {
@@ -287,12 +324,11 @@ private:
 
 // The kernel around the roles: barriers, TMEM, and the epilogue
 // `epi(smem, bars, tmem, warp of the epilogue, lane)`.
-template <int kTerms, int kRun, class Walk, class Epi>
+template <class S, int kRun, class Walk, class Epi>
 __device__ __forceinline__ void run_roles(const Walk &walk, Epi epi) {
-    using S = Shape<kTerms>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const Bars bars = bars_at<kTerms>(smem);
+    const Bars bars = bars_at<S>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     launch_dependents();
     if (threadIdx.x == 0) {
@@ -302,34 +338,42 @@ __device__ __forceinline__ void run_roles(const Walk &walk, Epi epi) {
         }
         for (int b = 0; b < 2; ++b) {
             tc::mbar_init(&bars.acc_full[b], 1);
-            tc::mbar_init(&bars.acc_empty[b], kEpiWarps);
+            tc::mbar_init(&bars.acc_empty[b], S::kCtas * kEpiWarps);
         }
         tc::fence_mbarrier_init();
     }
     if (warp == 1) {
-        tc::tmem_alloc(bars.tmem_slot, kTmemCols);
-        tc::tmem_relinquish();
+        if constexpr (S::kPair) {
+            tc::tmem_alloc_pair(bars.tmem_slot, kTmemCols);
+            tc::tmem_relinquish_pair();
+        } else {
+            tc::tmem_alloc(bars.tmem_slot, kTmemCols);
+            tc::tmem_relinquish();
+        }
     }
     tc::tc_fence_before();
-    __syncthreads();
+    if constexpr (S::kPair) tc::cluster_sync();  // the leader's barriers exist before the other CTA's loads
+    else __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = *bars.tmem_slot;
     grid_dependency_wait();
     if (warp < kFirstEpi) {
         tc::registers_down<kRoleRegisters>();
-        if (warp == 0) produce<kTerms, false>(smem, bars, walk);
-        if (warp == 2) produce<kTerms, true>(smem, bars, walk);
-        if (warp == 1) multiply<kTerms, kRun>(smem, bars, tmem, walk);
+        if (warp == 0) produce<S, false>(smem, bars, walk);
+        if (warp == 2) produce<S, true>(smem, bars, walk);
+        if (warp == 1 && tile_rank<S>() == 0) multiply<S, kRun>(smem, bars, tmem, walk);
         __syncwarp();
     } else {
         tc::registers_up<kEpiRegisters>();
         epi(smem, bars, tmem, warp, lane);
     }
     tc::tc_fence_before();
-    __syncthreads();
+    if constexpr (S::kPair) tc::cluster_sync();  // neither CTA leaves while the other may use its memory
+    else __syncthreads();
     if (warp == 1) {
         tc::tc_fence_after();
-        tc::tmem_dealloc(tmem, kTmemCols);
+        if constexpr (S::kPair) tc::tmem_dealloc_pair(tmem, kTmemCols);
+        else tc::tmem_dealloc(tmem, kTmemCols);
     }
 }
 
@@ -352,13 +396,14 @@ struct LogitArgs {
     float *target;    // [rows] logit of the label, in units of ln 2
     // backward
     const float *lse, *dloss;
-    float *column_sums;  // [4 m_tiles][count] or null
+    float *column_sums;  // [32-row blocks][count] or null
 };
 
 // The CTA's items, then each item's column tiles.  Items are row tiles in
 // groups of kGroupM, the items of a group by columns first, so that the CTAs
 // of a wave share kGroupM row tiles and few units.  32-bit arithmetic, two
 // divisions an item: the loading and the MMA lane walk between tiles.
+template <class S>
 struct LogitWalk {
     const LogitArgs &a;
     const CUtensorMap *map_x, *map_w;
@@ -366,7 +411,8 @@ struct LogitWalk {
     int m = 0, n = 0, end = 0;
 
     __device__ __forceinline__ LogitWalk(const LogitArgs &args, const CUtensorMap *x, const CUtensorMap *w)
-        : a(args), map_x(x), map_w(w), item(blockIdx.x), items(static_cast<uint32_t>(args.m_tiles) * args.splits) {}
+        : a(args), map_x(x), map_w(w), item(tile_group<S>()),
+          items(static_cast<uint32_t>(args.m_tiles) * args.splits) {}
     // Column tiles [n, end) of row tile m.
     __device__ __forceinline__ bool next_item() {
         if (item >= items) return false;
@@ -377,15 +423,17 @@ struct LogitWalk {
         m = static_cast<int>(group * kGroupM + rest - split * rows);
         n = static_cast<int>(split) * a.span;
         end = min(n + a.span, a.n_tiles);
-        item += gridDim.x;
+        item += tile_groups<S>();
         return true;
     }
+    // This CTA's 128 rows of row tile m.
+    __device__ __forceinline__ int block() const { return m * S::kCtas + static_cast<int>(tile_rank<S>()); }
     __device__ __forceinline__ bool next(Tile &t) {
         if (n == end && !next_item()) return false;
         t.a = map_x, t.b = map_w, t.a_mn = t.b_mn = false;
-        t.m0 = m * kTileM;
+        t.m0 = block() * kTileM;
         t.n0 = n * a.tile_n;  // map_w covers the launch's units
-        t.n_cols = min(a.tile_n, (a.count - t.n0 + 15) / 16 * 16);
+        t.n_cols = S::kPair ? S::kTileN : min(a.tile_n, (a.count - t.n0 + 15) / 16 * 16);
         t.k0 = 0;
         t.k1 = a.k_blocks;
         ++n;
@@ -393,29 +441,28 @@ struct LogitWalk {
     }
 };
 
-template <int kTerms, bool kBackward>
+template <class S, bool kBackward>
 __global__ void __launch_bounds__(kThreads, 1)
     logit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                  const __grid_constant__ CUtensorMap map_g, const LogitArgs a) {
-    using S = Shape<kTerms>;
-    const LogitWalk walk(a, &map_x, &map_w);
-    run_roles<kTerms, kShortRun>(walk, [&](uint8_t *smem, const Bars &bars, uint32_t tmem, int warp, int lane) {
+    constexpr int kTerms = S::kTerms;
+    const LogitWalk<S> walk(a, &map_x, &map_w);
+    run_roles<S, kShortRun>(walk, [&](uint8_t *smem, const Bars &bars, uint32_t tmem, int warp, int lane) {
         const int quarter = warp & 3, ew = warp - kFirstEpi, part = ew >> 2;
-        constexpr int kMax = Columns<kTerms, kShortRun>::kMax;
-        // 2 KB of the warp's own: a tile's bias first, then G on its way out
-        uint8_t *staging = smem + S::kStagingOff + ew * 2048;
+        constexpr int kMax = Columns<S, kShortRun>::kMax;
+        // the warp's own: a tile's bias first, then G on its way out
+        uint8_t *staging = smem + S::kStagingOff + ew * S::kStagingBytes;
         float *bias_slot = reinterpret_cast<float *>(staging);
         // a tile of 64 columns occupies two parts of 32
         const int part_cols = max(a.tile_n / kParts, 32), chunks = part * part_cols < a.tile_n ? part_cols / 32 : 0;
         const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * part_cols;
         // logits in units of ln 2, z log2(e): exponentials are powers of two
         const float2 scale = make_float2(a.scale * kLog2e, a.scale * kLog2e);
-        Columns<kTerms, kShortRun> columns;
+        Columns<S, kShortRun> columns;
         auto &v = columns.v;
-        LogitWalk own = walk;
+        LogitWalk<S> own = walk;
         while (own.next_item()) {
-            const int m = own.m;
-            const int64_t row = static_cast<int64_t>(m) * kTileM + quarter * 32 + lane;
+            const int64_t row0 = static_cast<int64_t>(own.block()) * kTileM + quarter * 32, row = row0 + lane;
             const bool live = row < a.rows;
             int32_t label = live ? a.labels[row] : -1;
             if (label >= a.k) label = -1;
@@ -548,14 +595,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 s[0] += __shfl_xor_sync(0xFFFFFFFFu, s[0], 16);
                                 const int c = col + h + lane;
                                 if (lane < 16 && c < a.count)
-                                    a.column_sums[(static_cast<int64_t>(m) * 4 + quarter) * a.count + c] = s[0];
+                                    a.column_sums[row0 / 32 * a.count + c] = s[0];
                             }
                         }
                         // G in bf16 (f32: three terms): a factor of its own
                         // products, rounded as any operand of theirs
 #pragma unroll
                         for (int p = 0; p < kTerms; ++p) {
-                            tc::bulk_wait_read<0>();
+                            if (S::kStoreCols == 32) tc::bulk_wait_read<0>();
                             __syncwarp();
 #pragma unroll
                             for (int c = 0; c < 4; ++c) {
@@ -571,15 +618,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                                         v[j][i + 1] -= f.y;
                                     }
                                 }
-                                // 64-byte rows, 16-byte units swizzled as SWIZZLE_64B expects
-                                *reinterpret_cast<uint4 *>(staging + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
-                                    make_uint4(w[0], w[1], w[2], w[3]);
+                                // 16-byte units swizzled as the store's map expects:
+                                // 64-byte rows as SWIZZLE_64B, 128-byte ones as SWIZZLE_128B
+                                const int at = S::kStoreCols == 32 ? lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)
+                                                                   : lane * 128 + (((4 * j + c) ^ (lane & 7)) << 4);
+                                *reinterpret_cast<uint4 *>(staging + at) = make_uint4(w[0], w[1], w[2], w[3]);
                             }
+                            if (S::kStoreCols == 64 && j + 1 < kMax) continue;
                             tc::fence_proxy_async_smem();
                             __syncwarp();
-                            const int64_t row0 = static_cast<int64_t>(m) * kTileM + quarter * 32;
-                            if (lane == 0 && col < a.count && row0 < a.rows) {
-                                tc::tma_store_3d(&map_g, staging, col, static_cast<int32_t>(row0), p);
+                            const int at = S::kStoreCols == 64 ? col0 : col;
+                            if (lane == 0 && at < a.count && row0 < a.rows) {
+                                tc::tma_store_3d(&map_g, staging, at, static_cast<int32_t>(row0), p);
                                 tc::bulk_commit();
                             }
                         }
@@ -654,6 +704,7 @@ struct ProductArgs {
 };
 
 // The CTA's items: the longer product's first.
+template <class S>
 struct ProductWalk {
     const ProductArgs &a;
     const CUtensorMap *map_g, *map_gt, *map_w, *map_x;
@@ -662,10 +713,10 @@ struct ProductWalk {
 
     __device__ __forceinline__ ProductWalk(const ProductArgs &args, const CUtensorMap *g, const CUtensorMap *gt,
                                            const CUtensorMap *w, const CUtensorMap *x)
-        : a(args), map_g(g), map_gt(gt), map_w(w), map_x(x), item(blockIdx.x) {}
+        : a(args), map_g(g), map_gt(gt), map_w(w), map_x(x), item(tile_group<S>()) {}
     __device__ __forceinline__ bool next_item() {
         uint32_t i = item;
-        item += gridDim.x;
+        item += tile_groups<S>();
         which = a.first_product;
         if (i >= a.one[which].items) {
             i -= a.one[which].items;
@@ -679,38 +730,40 @@ struct ProductWalk {
         m = static_cast<int>(rest) - split * a.one[which].m_tiles;
         return true;
     }
+    // This CTA's 128 rows of row tile m.
+    __device__ __forceinline__ int block() const { return m * S::kCtas + static_cast<int>(tile_rank<S>()); }
     __device__ __forceinline__ bool next(Tile &t) {
         if (!next_item()) return false;
         const auto &o = a.one[which];
         t.a = which == 0 ? map_g : map_gt, t.b = which == 0 ? map_w : map_x;
         t.a_mn = which == 1, t.b_mn = true;
-        t.m0 = m * kTileM;
+        t.m0 = block() * kTileM;
         t.n0 = n * a.tile_n;
-        t.n_cols = min(a.tile_n, (a.width - t.n0 + 15) / 16 * 16);
+        t.n_cols = S::kPair ? S::kTileN : min(a.tile_n, (a.width - t.n0 + 15) / 16 * 16);
         t.k0 = split * o.split_blocks;
         t.k1 = min(o.k_blocks, t.k0 + o.split_blocks);
         return true;
     }
 };
 
-template <int kTerms>
+template <class S>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_gt,
                    const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const ProductArgs a) {
-    const ProductWalk walk(a, &map_g, &map_gt, &map_w, &map_x);
-    constexpr int kRun = kTerms == 1 ? kOneRun : kShortRun;
-    run_roles<kTerms, kRun>(walk, [&](uint8_t *, const Bars &bars, uint32_t tmem, int warp, int lane) {
+    const ProductWalk<S> walk(a, &map_g, &map_gt, &map_w, &map_x);
+    constexpr int kRun = S::kTerms == 1 ? kOneRun : kShortRun;
+    run_roles<S, kRun>(walk, [&](uint8_t *, const Bars &bars, uint32_t tmem, int warp, int lane) {
         const int quarter = warp & 3, part = (warp - kFirstEpi) >> 2;
         const int part_cols = max(a.tile_n / kParts, 32), chunks = part * part_cols < a.tile_n ? part_cols / 32 : 0;
         const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * part_cols;
-        Columns<kTerms, kRun> columns;
-        ProductWalk p = walk;
+        Columns<S, kRun> columns;
+        ProductWalk<S> p = walk;
         while (p.next_item()) {
             const auto &o = a.one[p.which];
             const int k0 = p.split * o.split_blocks;
             columns.load(bars, base, min(o.k_blocks, k0 + o.split_blocks) - k0);
-            const int64_t row = static_cast<int64_t>(p.m) * kTileM + quarter * 32 + lane;
+            const int64_t row = static_cast<int64_t>(p.block()) * kTileM + quarter * 32 + lane;
             const float scale = columns.bad ? NAN : a.scale;
 #pragma unroll
             for (int j = 0; j < columns.kMax; ++j) {
@@ -927,13 +980,13 @@ CUtensorMap map_mn_major(const Terms &t, int cols) {
     const cuuint32_t box[4] = {64, kBlockK, static_cast<cuuint32_t>(cols / 64), 1};
     return encode(t, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-// G's stores: 32 by 32.
-CUtensorMap map_store(const Terms &t) {
+// G's stores: 32 rows by `cols` columns, 32 or 64.
+CUtensorMap map_store(const Terms &t, int cols) {
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(t.cols), static_cast<cuuint64_t>(t.rows),
                                 static_cast<cuuint64_t>(t.count)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(t.pitch) * 2, static_cast<cuuint64_t>(t.plane) * 2};
-    const cuuint32_t box[3] = {32, 32, 1};
-    return encode(t, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(cols), 32, 1};
+    return encode(t, 3, dims, strides, box, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // ---------------------------------------------------------------- plans
@@ -949,7 +1002,15 @@ int tile_columns(int64_t m_tiles, int64_t cols, int terms, int sms) {
     return n;
 }
 
+// Whether CTA pairs serve a product of so many rows and columns: full tiles
+// of 256 by 256 for two rounds of the pairs at least, and less than a quarter
+// of the columns' tiles empty.
+bool pairs_fit(int64_t rows, int64_t cols, int terms, int sms) {
+    return terms == 1 && ceil_div(rows, 256) * ceil_div(cols, 256) >= sms && ceil_div(cols, 256) * 192 <= cols;
+}
+
 struct ForwardPlan {
+    bool pair;
     int64_t m_tiles, n_tiles;
     int tile_n, span, splits;
     size_t xs, ws, partial, target, bytes;  // offsets
@@ -958,14 +1019,16 @@ struct ForwardPlan {
 ForwardPlan plan_forward(int64_t rows, int k, int width, int dtype, int sms) {
     const int terms = terms_of(dtype);
     ForwardPlan p{};
-    p.m_tiles = ceil_div(rows, kTileM);
-    p.tile_n = tile_columns(p.m_tiles, k, terms, sms);
+    p.pair = pairs_fit(rows, k, terms, sms);
+    const int groups = p.pair ? sms / 2 : sms;
+    p.m_tiles = ceil_div(rows, p.pair ? 2 * kTileM : kTileM);
+    p.tile_n = p.pair ? 256 : tile_columns(p.m_tiles, k, terms, sms);
     p.n_tiles = ceil_div(k, p.tile_n);
     // items of `span` column tiles: the fewest rounds of the grid, then the fewest items
     int64_t best = INT64_MAX;
     for (int64_t s = 1; s <= std::min<int64_t>(p.n_tiles, 64); ++s) {
         const int64_t span = ceil_div(p.n_tiles, s);
-        const int64_t cost = ceil_div(p.m_tiles * ceil_div(p.n_tiles, span), sms) * span;
+        const int64_t cost = ceil_div(p.m_tiles * ceil_div(p.n_tiles, span), groups) * span;
         if (cost < best) {
             best = cost;
             p.span = static_cast<int>(span);
@@ -989,7 +1052,7 @@ ForwardPlan plan_forward(int64_t rows, int k, int width, int dtype, int sms) {
 
 struct BackwardPlan {
     int64_t piece;  // units of a piece
-    int64_t m_tiles;
+    bool pair;      // the gradients' products (the logits' goes by the piece)
     int pitch, g_pitch, tile_n;  // tile_n: of the gradients' columns
     int splits[2];
     bool direct[2];
@@ -1003,12 +1066,14 @@ BackwardPlan plan_backward(int64_t rows, int k, int width, int dtype, int sms) {
     BackwardPlan p{};
     const int64_t fit = kPieceBytes / (std::max<int64_t>(rows, 1) * 2 * terms) / 256 * 256;
     p.piece = std::min<int64_t>(k, std::max<int64_t>(256, fit));
-    p.m_tiles = ceil_div(rows, kTileM);
     p.pitch = (width + 63) / 64 * 64;
     p.g_pitch = static_cast<int>((p.piece + 63) / 64 * 64);
     p.tile_n = width > 64 ? (terms == 1 && width > 128 ? 256 : 128) : 64;
     const int64_t n_tiles = ceil_div(width, p.tile_n);
-    const int64_t tiles[2] = {p.m_tiles * n_tiles, ceil_div(p.piece, kTileM) * n_tiles};
+    // both products' rows together: their depths keep the pairs busy
+    p.pair = p.tile_n == 256 && pairs_fit(rows + p.piece, width, terms, sms);
+    const int64_t tile_m = p.pair ? 2 * kTileM : kTileM, groups = p.pair ? sms / 2 : sms;
+    const int64_t tiles[2] = {ceil_div(rows, tile_m) * n_tiles, ceil_div(p.piece, tile_m) * n_tiles};
     const int64_t depth[2] = {ceil_div(p.piece, kBlockK), ceil_div(rows, kBlockK)};
     // Splits of the depth: the smallest round-robin makespan in depth blocks,
     // an item costing 6 more for its start and its epilogue and a split 4
@@ -1022,9 +1087,9 @@ BackwardPlan plan_backward(int64_t rows, int k, int width, int dtype, int sms) {
             const int64_t joined[2] = {ceil_div(depth[0], len[0]) > 1 ? 4 : 0, ceil_div(depth[1], len[1]) > 1 ? 4 : 0};
             const int64_t c[2] = {len[0] + 6 + joined[0], len[1] + 6 + joined[1]};
             int64_t cost = 0;
-            for (int64_t cta : {int64_t(0), n[f] % sms}) {
-                const int64_t own = n[f] > cta ? (n[f] - 1 - cta) / sms + 1 : 0;
-                const int64_t all = n[0] + n[1] > cta ? (n[0] + n[1] - 1 - cta) / sms + 1 : 0;
+            for (int64_t cta : {int64_t(0), n[f] % groups}) {
+                const int64_t own = n[f] > cta ? (n[f] - 1 - cta) / groups + 1 : 0;
+                const int64_t all = n[0] + n[1] > cta ? (n[0] + n[1] - 1 - cta) / groups + 1 : 0;
                 cost = std::max(cost, own * c[f] + (all - own) * c[f ^ 1]);
             }
             cost = cost * 8 + joined[0] + joined[1];
@@ -1045,7 +1110,7 @@ BackwardPlan plan_backward(int64_t rows, int k, int width, int dtype, int sms) {
     p.xs = put(static_cast<size_t>(terms) * rows * p.pitch * 2);
     p.ws = put(static_cast<size_t>(terms) * k * p.pitch * 2);
     p.g = put(static_cast<size_t>(terms) * rows * p.g_pitch * 2);
-    p.sums = put(static_cast<size_t>(4) * p.m_tiles * p.piece * sizeof(float));
+    p.sums = put(static_cast<size_t>(ceil_div(rows, 256)) * 8 * p.piece * sizeof(float));  // rows of whole pair tiles
     p.part[0] = put(p.direct[0] ? 0 : static_cast<size_t>(p.splits[0]) * rows * width * sizeof(float));
     p.part[1] = put(p.direct[1] ? 0 : static_cast<size_t>(p.splits[1]) * p.piece * width * sizeof(float));
     p.bytes = at;
@@ -1063,13 +1128,35 @@ void allow_smem() {
     auto allow = [](auto kernel, size_t bytes) {
         cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
     };
-    allow(logit_kernel<1, false>, Shape<1>::kSmem);
-    allow(logit_kernel<1, true>, Shape<1>::kSmem);
-    allow(product_kernel<1>, Shape<1>::kSmem);
-    allow(logit_kernel<3, false>, Shape<3>::kSmem);
-    allow(logit_kernel<3, true>, Shape<3>::kSmem);
-    allow(product_kernel<3>, Shape<3>::kSmem);
+    auto shape = [&](auto s) {
+        using S = decltype(s);
+        allow(logit_kernel<S, false>, S::kSmem);
+        allow(logit_kernel<S, true>, S::kSmem);
+        allow(product_kernel<S>, S::kSmem);
+    };
+    shape(Shape<1, false>{});
+    shape(Shape<1, true>{});
+    shape(Shape<3, false>{});
     if (device < 64) done |= uint64_t(1) << device;
+}
+
+// Launches a product kernel of shape S with `groups` CTAs or pairs.
+template <class S, class Kernel, class... Args>
+void launch_groups(Kernel kernel, int64_t groups, cudaStream_t stream, const Args &...args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(groups * S::kCtas));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = S::kPair ? 2 : 1;
+    cuda_check(cudaLaunchKernelEx(&cfg, kernel, args...));
 }
 
 bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -1096,7 +1183,7 @@ void forward(const UnitLoss &a, int sms, cudaStream_t stream) {
         x = xs, w = ws, pitch = p.pitch;
     }
     const CUtensorMap map_x = map_k_major({x, a.width, a.rows, pitch, a.rows * pitch, kTerms}, kTileM);
-    const CUtensorMap map_w = map_k_major({w, a.width, a.k, pitch, a.k * pitch, kTerms}, p.tile_n);
+    const CUtensorMap map_w = map_k_major({w, a.width, a.k, pitch, a.k * pitch, kTerms}, p.pair ? 128 : p.tile_n);
     LogitArgs l{};
     l.rows = a.rows, l.first = 0, l.count = a.k, l.k = a.k;
     l.k_blocks = static_cast<int32_t>(ceil_div(a.width, kBlockK));
@@ -1106,9 +1193,17 @@ void forward(const UnitLoss &a, int sms, cudaStream_t stream) {
     l.partial = reinterpret_cast<float2 *>(base + p.partial);
     l.target = reinterpret_cast<float *>(base + p.target);
     allow_smem();
-    const int64_t grid = std::min<int64_t>(p.m_tiles * p.splits, sms);
-    cuda_check(launch_pdl(logit_kernel<kTerms, false>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
-                          Shape<kTerms>::kSmem, stream, map_x, map_w, map_x, l));
+    if (p.pair) {
+        if constexpr (kTerms == 1) {
+            using S = Shape<1, true>;
+            launch_groups<S>(logit_kernel<S, false>, std::min<int64_t>(p.m_tiles * p.splits, sms / 2), stream, map_x,
+                             map_w, map_x, l);
+        }
+    } else {
+        using S = Shape<kTerms, false>;
+        launch_groups<S>(logit_kernel<S, false>, std::min<int64_t>(p.m_tiles * p.splits, sms), stream, map_x, map_w,
+                         map_x, l);
+    }
     cuda_check(launch_pdl(loss_kernel, dim3(static_cast<unsigned>(ceil_div(a.rows, 32))), dim3(256), 0, stream,
                           static_cast<const float2 *>(l.partial), static_cast<const float *>(l.target), a.labels,
                           a.rows, kParts * p.splits, static_cast<int>(a.k), a.loss, a.lse));
@@ -1123,7 +1218,7 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
     stage<T, kTerms>(a, p.pitch, true, xs, ws, sms, stream);
     const int64_t pitch = p.pitch, plane = a.k * pitch;
     const Terms x{xs, a.width, a.rows, pitch, a.rows * pitch, kTerms};
-    const CUtensorMap map_x = map_k_major(x, kTileM), map_xt = map_mn_major(x, p.tile_n);
+    const CUtensorMap map_x = map_k_major(x, kTileM), map_xt = map_mn_major(x, p.pair ? 128 : p.tile_n);
     allow_smem();
     for (int64_t first = 0; first < a.k; first += p.piece) {
         const int64_t count = std::min<int64_t>(p.piece, a.k - first);
@@ -1132,17 +1227,26 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
         LogitArgs l{};
         l.rows = a.rows, l.first = static_cast<int32_t>(first), l.count = static_cast<int32_t>(count), l.k = a.k;
         l.k_blocks = static_cast<int32_t>(ceil_div(a.width, kBlockK));
-        l.m_tiles = static_cast<int32_t>(p.m_tiles);
-        l.tile_n = tile_columns(p.m_tiles, count, kTerms, sms);
+        const bool pair = pairs_fit(a.rows, count, kTerms, sms);
+        l.m_tiles = static_cast<int32_t>(ceil_div(a.rows, pair ? 2 * kTileM : kTileM));
+        l.tile_n = pair ? 256 : tile_columns(l.m_tiles, count, kTerms, sms);
         l.n_tiles = l.splits = static_cast<int32_t>(ceil_div(count, l.tile_n));
         l.span = 1;
         l.bias = a.bias, l.labels = a.labels, l.scale = a.scale;
         l.lse = a.lse_in, l.dloss = a.dloss;
         l.column_sums = a.dbias ? reinterpret_cast<float *>(base + p.sums) : nullptr;
-        int64_t grid = std::min<int64_t>(p.m_tiles * l.splits, sms);
-        cuda_check(launch_pdl(logit_kernel<kTerms, true>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
-                              Shape<kTerms>::kSmem, stream, map_x, map_k_major(w, l.tile_n),
-                              map_store(g), l));
+        const int64_t items = static_cast<int64_t>(l.m_tiles) * l.splits;
+        if (pair) {
+            if constexpr (kTerms == 1) {
+                using S = Shape<1, true>;
+                launch_groups<S>(logit_kernel<S, true>, std::min<int64_t>(items, sms / 2), stream, map_x,
+                                 map_k_major(w, 128), map_store(g, S::kStoreCols), l);
+            }
+        } else {
+            using S = Shape<kTerms, false>;
+            launch_groups<S>(logit_kernel<S, true>, std::min<int64_t>(items, sms), stream, map_x,
+                             map_k_major(w, l.tile_n), map_store(g, S::kStoreCols), l);
+        }
         ProductArgs q{};
         q.width = a.width, q.tile_n = p.tile_n;
         q.n_tiles = static_cast<int32_t>(ceil_div(a.width, p.tile_n));
@@ -1155,7 +1259,7 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
         for (int i = 0; i < 2; ++i) {
             auto &o = q.one[i];
             o.m_size = static_cast<int32_t>(size[i]);
-            o.m_tiles = static_cast<int32_t>(ceil_div(size[i], kTileM));
+            o.m_tiles = static_cast<int32_t>(ceil_div(size[i], p.pair ? 2 * kTileM : kTileM));
             o.k_blocks = static_cast<int32_t>(depth[i]);
             // the last piece is shorter: its splits are too, and all of them exist
             o.splits = static_cast<int32_t>(std::min<int64_t>(p.splits[i], depth[i]));
@@ -1168,10 +1272,18 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
             o.part_stride = size[i] * a.width;
         }
         q.first_product = q.one[0].split_blocks >= q.one[1].split_blocks ? 0 : 1;
-        grid = std::min<int64_t>(q.one[0].items + q.one[1].items, sms);
-        cuda_check(launch_pdl(product_kernel<kTerms>, dim3(static_cast<unsigned>(grid)), dim3(kThreads),
-                              Shape<kTerms>::kSmem, stream, map_k_major(g, kTileM),
-                              map_mn_major(g, kTileM), map_mn_major(w, p.tile_n), map_xt, q));
+        const int64_t tiles = static_cast<int64_t>(q.one[0].items) + q.one[1].items;
+        if (p.pair) {
+            if constexpr (kTerms == 1) {
+                using S = Shape<1, true>;
+                launch_groups<S>(product_kernel<S>, std::min<int64_t>(tiles, sms / 2), stream, map_k_major(g, kTileM),
+                                 map_mn_major(g, kTileM), map_mn_major(w, 128), map_xt, q);
+            }
+        } else {
+            using S = Shape<kTerms, false>;
+            launch_groups<S>(product_kernel<S>, std::min<int64_t>(tiles, sms), stream, map_k_major(g, kTileM),
+                             map_mn_major(g, kTileM), map_mn_major(w, p.tile_n), map_xt, q);
+        }
         auto join = [&](int i) {
             const auto &o = q.one[i];
             const int64_t n = size[i] * a.width;
@@ -1185,7 +1297,7 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
         if (!p.direct[0] && first + count == a.k) join(0);
         if (a.dbias)
             cuda_check(launch_pdl(dbias_kernel, dim3(static_cast<unsigned>(ceil_div(count, 32))), dim3(1024), 0,
-                                  stream, static_cast<const float *>(l.column_sums), 4 * p.m_tiles,
+                                  stream, static_cast<const float *>(l.column_sums), ceil_div(a.rows, 32),
                                   static_cast<int32_t>(count), a.dbias + first));
     }
 }
