@@ -63,8 +63,9 @@ __device__ __forceinline__ float exp2_approx(float v) {
 // holds the tile's rows 128 r .. of A and columns 128 r .. of B at the same
 // offsets as the other, and its TMEM gets its rows of the result: 32 KB a
 // stage and CTA where one CTA alone reads 48 KB, so that L2 keeps up, and
-// five stages.  The even CTA leads: it issues the MMAs, and every load of a
-// stage counts on its barrier.
+// six stages.  The even CTA leads: it issues the MMAs, and every load of a
+// stage counts on its barrier.  The gradients' products take it; the logits'
+// do not: their epilogues would hold up two CTAs at a time.
 template <int kTerms_, bool kPair_>
 struct Shape {
     static constexpr int kTerms = kTerms_;
@@ -72,13 +73,12 @@ struct Shape {
     static_assert(!kPair || kTerms == 1, "pairs multiply bf16");
     static constexpr int kCtas = kPair ? 2 : 1;
     static constexpr int kTileN = kTerms == 1 ? 256 : 128;
-    static constexpr int kStages = kPair ? 5 : kTerms == 1 ? 4 : 2;
+    static constexpr int kStages = kPair ? 6 : kTerms == 1 ? 4 : 2;
     static constexpr uint32_t kABytes = 2 * kBoxBytes;
     static constexpr uint32_t kBBytes = kTileN / kCtas / 64 * kBoxBytes;
     static constexpr uint32_t kStageBytes = kTerms * (kABytes + kBBytes);
-    // G on its way out, per epilogue warp: 32 rows of 32 columns, of a pair 64
-    static constexpr int kStoreCols = kPair ? 64 : 32;
-    static constexpr uint32_t kStagingBytes = 32 * kStoreCols * 2;
+    // G on its way out, per epilogue warp: 32 rows of 32 columns
+    static constexpr uint32_t kStagingBytes = 32 * 32 * 2;
     static constexpr uint32_t kStagingOff = kStages * kStageBytes;
     static constexpr uint32_t kBarOff = kStagingOff + kEpiWarps * kStagingBytes;
     static constexpr size_t kSmem = 1024 + kBarOff + 256;
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         // products, rounded as any operand of theirs
 #pragma unroll
                         for (int p = 0; p < kTerms; ++p) {
-                            if (S::kStoreCols == 32) tc::bulk_wait_read<0>();
+                            tc::bulk_wait_read<0>();
                             __syncwarp();
 #pragma unroll
                             for (int c = 0; c < 4; ++c) {
@@ -618,18 +618,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                                         v[j][i + 1] -= f.y;
                                     }
                                 }
-                                // 16-byte units swizzled as the store's map expects:
-                                // 64-byte rows as SWIZZLE_64B, 128-byte ones as SWIZZLE_128B
-                                const int at = S::kStoreCols == 32 ? lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)
-                                                                   : lane * 128 + (((4 * j + c) ^ (lane & 7)) << 4);
-                                *reinterpret_cast<uint4 *>(staging + at) = make_uint4(w[0], w[1], w[2], w[3]);
+                                // 64-byte rows, 16-byte units swizzled as SWIZZLE_64B expects
+                                *reinterpret_cast<uint4 *>(staging + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+                                    make_uint4(w[0], w[1], w[2], w[3]);
                             }
-                            if (S::kStoreCols == 64 && j + 1 < kMax) continue;
                             tc::fence_proxy_async_smem();
                             __syncwarp();
-                            const int at = S::kStoreCols == 64 ? col0 : col;
-                            if (lane == 0 && at < a.count && row0 < a.rows) {
-                                tc::tma_store_3d(&map_g, staging, at, static_cast<int32_t>(row0), p);
+                            if (lane == 0 && col < a.count && row0 < a.rows) {
+                                tc::tma_store_3d(&map_g, staging, col, static_cast<int32_t>(row0), p);
                                 tc::bulk_commit();
                             }
                         }
@@ -699,16 +695,19 @@ struct ProductArgs {
     } one[2];
     int32_t width, n_tiles, tile_n;
     int32_t first_product;  // whose items come first: the longer ones
+    uint32_t odd, extra;    // see ProductWalk
     float scale;
     bool bf16, wide;        // result type; 16-byte stores fit
 };
 
-// The CTA's items: the longer product's first.
+// The CTA's items: the longer product's in turn over the grid, then the
+// other's.  Where the longer ones do not come out even, the CTAs that got one
+// less (from `odd` on) first take `extra` short items each.
 template <class S>
 struct ProductWalk {
     const ProductArgs &a;
     const CUtensorMap *map_g, *map_gt, *map_w, *map_x;
-    uint32_t item;
+    uint32_t item, taken = 0;  // next long item; short items taken
     int which = 0, m = 0, n = 0, split = 0;
 
     __device__ __forceinline__ ProductWalk(const ProductArgs &args, const CUtensorMap *g, const CUtensorMap *gt,
@@ -716,11 +715,19 @@ struct ProductWalk {
         : a(args), map_g(g), map_gt(gt), map_w(w), map_x(x), item(tile_group<S>()) {}
     __device__ __forceinline__ bool next_item() {
         uint32_t i = item;
-        item += tile_groups<S>();
         which = a.first_product;
-        if (i >= a.one[which].items) {
-            i -= a.one[which].items;
+        if (i < a.one[which].items) {
+            item += tile_groups<S>();
+        } else {
             which ^= 1;
+            const uint32_t groups = tile_groups<S>(), own = tile_group<S>(), late = groups - a.odd;
+            if (own >= a.odd && taken < a.extra) {
+                i = taken * late + own - a.odd;
+            } else {
+                const uint32_t round = own >= a.odd ? taken - a.extra : taken;
+                i = a.extra * late + round * groups + own;
+            }
+            ++taken;
             if (i >= a.one[which].items) return false;
         }
         // columns first, then splits: neighbours share their rows of G
@@ -980,13 +987,13 @@ CUtensorMap map_mn_major(const Terms &t, int cols) {
     const cuuint32_t box[4] = {64, kBlockK, static_cast<cuuint32_t>(cols / 64), 1};
     return encode(t, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-// G's stores: 32 rows by `cols` columns, 32 or 64.
-CUtensorMap map_store(const Terms &t, int cols) {
+// G's stores: 32 by 32.
+CUtensorMap map_store(const Terms &t) {
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(t.cols), static_cast<cuuint64_t>(t.rows),
                                 static_cast<cuuint64_t>(t.count)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(t.pitch) * 2, static_cast<cuuint64_t>(t.plane) * 2};
-    const cuuint32_t box[3] = {static_cast<cuuint32_t>(cols), 32, 1};
-    return encode(t, 3, dims, strides, box, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+    const cuuint32_t box[3] = {32, 32, 1};
+    return encode(t, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // ---------------------------------------------------------------- plans
@@ -1009,8 +1016,21 @@ bool pairs_fit(int64_t rows, int64_t cols, int terms, int sms) {
     return terms == 1 && ceil_div(rows, 256) * ceil_div(cols, 256) >= sms && ceil_div(cols, 256) * 192 <= cols;
 }
 
+// Column tiles of an item: the fewest rounds of the grid, then the fewest items.
+int item_span(int64_t m_tiles, int64_t n_tiles, int sms) {
+    int64_t best = INT64_MAX, span = 1;
+    for (int64_t s = 1; s <= std::min<int64_t>(n_tiles, 64); ++s) {
+        const int64_t each = ceil_div(n_tiles, s);
+        const int64_t cost = ceil_div(m_tiles * ceil_div(n_tiles, each), sms) * each;
+        if (cost < best) {
+            best = cost;
+            span = each;
+        }
+    }
+    return static_cast<int>(span);
+}
+
 struct ForwardPlan {
-    bool pair;
     int64_t m_tiles, n_tiles;
     int tile_n, span, splits;
     size_t xs, ws, partial, target, bytes;  // offsets
@@ -1019,21 +1039,10 @@ struct ForwardPlan {
 ForwardPlan plan_forward(int64_t rows, int k, int width, int dtype, int sms) {
     const int terms = terms_of(dtype);
     ForwardPlan p{};
-    p.pair = pairs_fit(rows, k, terms, sms);
-    const int groups = p.pair ? sms / 2 : sms;
-    p.m_tiles = ceil_div(rows, p.pair ? 2 * kTileM : kTileM);
-    p.tile_n = p.pair ? 256 : tile_columns(p.m_tiles, k, terms, sms);
+    p.m_tiles = ceil_div(rows, kTileM);
+    p.tile_n = tile_columns(p.m_tiles, k, terms, sms);
     p.n_tiles = ceil_div(k, p.tile_n);
-    // items of `span` column tiles: the fewest rounds of the grid, then the fewest items
-    int64_t best = INT64_MAX;
-    for (int64_t s = 1; s <= std::min<int64_t>(p.n_tiles, 64); ++s) {
-        const int64_t span = ceil_div(p.n_tiles, s);
-        const int64_t cost = ceil_div(p.m_tiles * ceil_div(p.n_tiles, span), groups) * span;
-        if (cost < best) {
-            best = cost;
-            p.span = static_cast<int>(span);
-        }
-    }
+    p.span = item_span(p.m_tiles, p.n_tiles, sms);
     p.splits = static_cast<int>(ceil_div(p.n_tiles, p.span));
     p.pitch = (width + 63) / 64 * 64;
     size_t at = 0;
@@ -1048,6 +1057,26 @@ ForwardPlan plan_forward(int64_t rows, int k, int width, int dtype, int sms) {
     p.target = put(static_cast<size_t>(rows) * sizeof(float));
     p.bytes = at;
     return p;
+}
+
+// How many short items (of cost `brief`) the groups that got one long item
+// (of cost `slow`) less take first, for the smallest makespan.
+int64_t even_out(int64_t slows, int64_t briefs, int64_t slow, int64_t brief, int64_t groups, int64_t *makespan) {
+    const int64_t odd = slows % groups, late = groups - odd, each = slows / groups;
+    int64_t best = INT64_MAX, extra = 0;
+    const int64_t most = odd ? slow / brief + 1 : 0;
+    for (int64_t e = std::max<int64_t>(0, most - 1); e <= most; ++e) {
+        const int64_t rest = briefs - e * late;
+        const int64_t rounds = rest > 0 ? ceil_div(rest, groups) : 0;
+        const int64_t early = (each + (odd ? 1 : 0)) * slow + rounds * brief;
+        const int64_t other = each * slow + (rest > 0 ? e + rounds : ceil_div(briefs, late)) * brief;
+        if (std::max(early, other) < best) {
+            best = std::max(early, other);
+            extra = e;
+        }
+    }
+    *makespan = best;
+    return extra;
 }
 
 struct BackwardPlan {
@@ -1075,28 +1104,25 @@ BackwardPlan plan_backward(int64_t rows, int k, int width, int dtype, int sms) {
     const int64_t tile_m = p.pair ? 2 * kTileM : kTileM, groups = p.pair ? sms / 2 : sms;
     const int64_t tiles[2] = {ceil_div(rows, tile_m) * n_tiles, ceil_div(p.piece, tile_m) * n_tiles};
     const int64_t depth[2] = {ceil_div(p.piece, kBlockK), ceil_div(rows, kBlockK)};
-    // Splits of the depth: the smallest round-robin makespan in depth blocks,
-    // an item costing 6 more for its start and its epilogue and a split 4
-    // more for the join.
+    // Splits of the depth: the smallest makespan in depth blocks, an item
+    // costing 6 more for its start and its epilogue and a split 8 more for
+    // the join; then the least to join.
     int64_t best = INT64_MAX;
     for (int s0 = 1; s0 <= 64 && s0 <= depth[0]; s0 = s0 < 4 ? s0 + 1 : s0 * 2)
         for (int s1 = 1; s1 <= 64 && s1 <= depth[1]; s1 = s1 < 4 ? s1 + 1 : s1 * 2) {
             const int64_t len[2] = {ceil_div(depth[0], s0), ceil_div(depth[1], s1)};
+            const int64_t splits[2] = {ceil_div(depth[0], len[0]), ceil_div(depth[1], len[1])};
+            const int64_t n[2] = {tiles[0] * splits[0], tiles[1] * splits[1]};
+            const int64_t c[2] = {len[0] + 6 + (splits[0] > 1 ? 8 : 0), len[1] + 6 + (splits[1] > 1 ? 8 : 0)};
             const int f = len[0] >= len[1] ? 0 : 1;
-            const int64_t n[2] = {tiles[0] * ceil_div(depth[0], len[0]), tiles[1] * ceil_div(depth[1], len[1])};
-            const int64_t joined[2] = {ceil_div(depth[0], len[0]) > 1 ? 4 : 0, ceil_div(depth[1], len[1]) > 1 ? 4 : 0};
-            const int64_t c[2] = {len[0] + 6 + joined[0], len[1] + 6 + joined[1]};
             int64_t cost = 0;
-            for (int64_t cta : {int64_t(0), n[f] % groups}) {
-                const int64_t own = n[f] > cta ? (n[f] - 1 - cta) / groups + 1 : 0;
-                const int64_t all = n[0] + n[1] > cta ? (n[0] + n[1] - 1 - cta) / groups + 1 : 0;
-                cost = std::max(cost, own * c[f] + (all - own) * c[f ^ 1]);
-            }
-            cost = cost * 8 + joined[0] + joined[1];
+            even_out(n[f], n[f ^ 1], c[f], c[f ^ 1], groups, &cost);
+            // what is joined crosses HBM twice in f32: 1 depth block's time for 2 tiles or so
+            cost += ((splits[0] > 1 ? n[0] : 0) + (splits[1] > 1 ? n[1] : 0)) / 16;
             if (cost < best) {
                 best = cost;
-                p.splits[0] = static_cast<int>(ceil_div(depth[0], len[0]));
-                p.splits[1] = static_cast<int>(ceil_div(depth[1], len[1]));
+                p.splits[0] = static_cast<int>(splits[0]);
+                p.splits[1] = static_cast<int>(splits[1]);
             }
         }
     p.direct[0] = p.splits[0] == 1 && p.piece == k;
@@ -1135,8 +1161,8 @@ void allow_smem() {
         allow(product_kernel<S>, S::kSmem);
     };
     shape(Shape<1, false>{});
-    shape(Shape<1, true>{});
     shape(Shape<3, false>{});
+    allow(product_kernel<Shape<1, true>>, Shape<1, true>::kSmem);
     if (device < 64) done |= uint64_t(1) << device;
 }
 
@@ -1183,7 +1209,7 @@ void forward(const UnitLoss &a, int sms, cudaStream_t stream) {
         x = xs, w = ws, pitch = p.pitch;
     }
     const CUtensorMap map_x = map_k_major({x, a.width, a.rows, pitch, a.rows * pitch, kTerms}, kTileM);
-    const CUtensorMap map_w = map_k_major({w, a.width, a.k, pitch, a.k * pitch, kTerms}, p.pair ? 128 : p.tile_n);
+    const CUtensorMap map_w = map_k_major({w, a.width, a.k, pitch, a.k * pitch, kTerms}, p.tile_n);
     LogitArgs l{};
     l.rows = a.rows, l.first = 0, l.count = a.k, l.k = a.k;
     l.k_blocks = static_cast<int32_t>(ceil_div(a.width, kBlockK));
@@ -1193,17 +1219,9 @@ void forward(const UnitLoss &a, int sms, cudaStream_t stream) {
     l.partial = reinterpret_cast<float2 *>(base + p.partial);
     l.target = reinterpret_cast<float *>(base + p.target);
     allow_smem();
-    if (p.pair) {
-        if constexpr (kTerms == 1) {
-            using S = Shape<1, true>;
-            launch_groups<S>(logit_kernel<S, false>, std::min<int64_t>(p.m_tiles * p.splits, sms / 2), stream, map_x,
-                             map_w, map_x, l);
-        }
-    } else {
-        using S = Shape<kTerms, false>;
-        launch_groups<S>(logit_kernel<S, false>, std::min<int64_t>(p.m_tiles * p.splits, sms), stream, map_x, map_w,
-                         map_x, l);
-    }
+    using S = Shape<kTerms, false>;
+    launch_groups<S>(logit_kernel<S, false>, std::min<int64_t>(p.m_tiles * p.splits, sms), stream, map_x, map_w, map_x,
+                     l);
     cuda_check(launch_pdl(loss_kernel, dim3(static_cast<unsigned>(ceil_div(a.rows, 32))), dim3(256), 0, stream,
                           static_cast<const float2 *>(l.partial), static_cast<const float *>(l.target), a.labels,
                           a.rows, kParts * p.splits, static_cast<int>(a.k), a.loss, a.lse));
@@ -1227,25 +1245,19 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
         LogitArgs l{};
         l.rows = a.rows, l.first = static_cast<int32_t>(first), l.count = static_cast<int32_t>(count), l.k = a.k;
         l.k_blocks = static_cast<int32_t>(ceil_div(a.width, kBlockK));
-        const bool pair = pairs_fit(a.rows, count, kTerms, sms);
-        l.m_tiles = static_cast<int32_t>(ceil_div(a.rows, pair ? 2 * kTileM : kTileM));
-        l.tile_n = pair ? 256 : tile_columns(l.m_tiles, count, kTerms, sms);
-        l.n_tiles = l.splits = static_cast<int32_t>(ceil_div(count, l.tile_n));
-        l.span = 1;
+        l.m_tiles = static_cast<int32_t>(ceil_div(a.rows, kTileM));
+        l.tile_n = tile_columns(l.m_tiles, count, kTerms, sms);
+        l.n_tiles = static_cast<int32_t>(ceil_div(count, l.tile_n));
+        l.span = item_span(l.m_tiles, l.n_tiles, sms);
+        l.splits = static_cast<int32_t>(ceil_div(l.n_tiles, l.span));
         l.bias = a.bias, l.labels = a.labels, l.scale = a.scale;
         l.lse = a.lse_in, l.dloss = a.dloss;
         l.column_sums = a.dbias ? reinterpret_cast<float *>(base + p.sums) : nullptr;
-        const int64_t items = static_cast<int64_t>(l.m_tiles) * l.splits;
-        if (pair) {
-            if constexpr (kTerms == 1) {
-                using S = Shape<1, true>;
-                launch_groups<S>(logit_kernel<S, true>, std::min<int64_t>(items, sms / 2), stream, map_x,
-                                 map_k_major(w, 128), map_store(g, S::kStoreCols), l);
-            }
-        } else {
+        {
             using S = Shape<kTerms, false>;
-            launch_groups<S>(logit_kernel<S, true>, std::min<int64_t>(items, sms), stream, map_x,
-                             map_k_major(w, l.tile_n), map_store(g, S::kStoreCols), l);
+            launch_groups<S>(logit_kernel<S, true>,
+                             std::min<int64_t>(static_cast<int64_t>(l.m_tiles) * l.splits, sms), stream, map_x,
+                             map_k_major(w, l.tile_n), map_store(g), l);
         }
         ProductArgs q{};
         q.width = a.width, q.tile_n = p.tile_n;
@@ -1273,15 +1285,21 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
         }
         q.first_product = q.one[0].split_blocks >= q.one[1].split_blocks ? 0 : 1;
         const int64_t tiles = static_cast<int64_t>(q.one[0].items) + q.one[1].items;
+        const int64_t groups = std::min<int64_t>(tiles, p.pair ? sms / 2 : sms);
+        const auto &slow = q.one[q.first_product], &brief = q.one[q.first_product ^ 1];
+        int64_t makespan = 0;
+        q.odd = static_cast<uint32_t>(slow.items % groups);
+        q.extra = static_cast<uint32_t>(
+            even_out(slow.items, brief.items, slow.split_blocks + 6, brief.split_blocks + 6, groups, &makespan));
         if (p.pair) {
             if constexpr (kTerms == 1) {
                 using S = Shape<1, true>;
-                launch_groups<S>(product_kernel<S>, std::min<int64_t>(tiles, sms / 2), stream, map_k_major(g, kTileM),
+                launch_groups<S>(product_kernel<S>, groups, stream, map_k_major(g, kTileM),
                                  map_mn_major(g, kTileM), map_mn_major(w, 128), map_xt, q);
             }
         } else {
             using S = Shape<kTerms, false>;
-            launch_groups<S>(product_kernel<S>, std::min<int64_t>(tiles, sms), stream, map_k_major(g, kTileM),
+            launch_groups<S>(product_kernel<S>, groups, stream, map_k_major(g, kTileM),
                              map_mn_major(g, kTileM), map_mn_major(w, p.tile_n), map_xt, q);
         }
         auto join = [&](int i) {
