@@ -73,14 +73,16 @@ struct Shape {
     static_assert(!kPair || kTerms == 1, "pairs multiply bf16");
     static constexpr int kCtas = kPair ? 2 : 1;
     static constexpr int kTileN = kTerms == 1 ? 256 : 128;
-    static constexpr int kStages = kPair ? 6 : kTerms == 1 ? 4 : 2;
+    static constexpr int kStages = kPair ? 6 : kTerms == 1 ? 3 : 2;
     static constexpr uint32_t kABytes = 2 * kBoxBytes;
     static constexpr uint32_t kBBytes = kTileN / kCtas / 64 * kBoxBytes;
     static constexpr uint32_t kStageBytes = kTerms * (kABytes + kBBytes);
     // G on its way out, per epilogue warp: 32 rows of 32 columns
-    static constexpr uint32_t kStagingBytes = 32 * 32 * 2;
+    static constexpr int kBuffers = kTerms == 1 && !kPair ? 2 : 1;
+    static constexpr uint32_t kStagingBytes = kBuffers * 32 * 32 * 2;
     static constexpr uint32_t kStagingOff = kStages * kStageBytes;
-    static constexpr uint32_t kBarOff = kStagingOff + kEpiWarps * kStagingBytes;
+    static constexpr uint32_t kBiasOff = kStagingOff + kEpiWarps * kStagingBytes;
+    static constexpr uint32_t kBarOff = kBiasOff + (kBuffers == 2 ? kEpiWarps * 256 : 0);
     static constexpr size_t kSmem = 1024 + kBarOff + 256;
     static_assert(kSmem <= 232448, "shared memory");
 };
@@ -452,7 +454,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr int kMax = Columns<S, kShortRun>::kMax;
         // the warp's own: a tile's bias first, then G on its way out
         uint8_t *staging = smem + S::kStagingOff + ew * S::kStagingBytes;
-        float *bias_slot = reinterpret_cast<float *>(staging);
+        float *bias_slot = reinterpret_cast<float *>(S::kBuffers == 2 ? smem + S::kBiasOff + ew * 256 : staging);
+        uint32_t stores = 0;
         // a tile of 64 columns occupies two parts of 32
         const int part_cols = max(a.tile_n / kParts, 32), chunks = part * part_cols < a.tile_n ? part_cols / 32 : 0;
         const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * part_cols;
@@ -481,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // bias of the part's columns, and which take no part: units
                 // left out and columns past the last
                 uint32_t out[kMax];
-                if constexpr (kBackward) tc::bulk_wait_read<0>();
+                if constexpr (kBackward && S::kBuffers == 1) tc::bulk_wait_read<0>();
                 __syncwarp();
 #pragma unroll
                 for (int j = 0; j < kMax; ++j) {
@@ -602,8 +605,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         // products, rounded as any operand of theirs
 #pragma unroll
                         for (int p = 0; p < kTerms; ++p) {
-                            tc::bulk_wait_read<0>();
+                            tc::bulk_wait_read<S::kBuffers - 1>();
                             __syncwarp();
+                            uint8_t *buf = staging + (S::kBuffers == 2 ? (stores++ & 1) * 2048 : 0);
 #pragma unroll
                             for (int c = 0; c < 4; ++c) {
                                 uint32_t w[4];
@@ -619,15 +623,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     }
                                 }
                                 // 64-byte rows, 16-byte units swizzled as SWIZZLE_64B expects
-                                *reinterpret_cast<uint4 *>(staging + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
+                                *reinterpret_cast<uint4 *>(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
                                     make_uint4(w[0], w[1], w[2], w[3]);
                             }
                             tc::fence_proxy_async_smem();
                             __syncwarp();
-                            if (lane == 0 && col < a.count && row0 < a.rows) {
-                                tc::tma_store_3d(&map_g, staging, col, static_cast<int32_t>(row0), p);
-                                tc::bulk_commit();
-                            }
+                            if (lane == 0 && col < a.count && row0 < a.rows)
+                                tc::tma_store_3d(&map_g, buf, col, static_cast<int32_t>(row0), p);
+                            if (lane == 0) tc::bulk_commit();
                         }
                     }
                 }
