@@ -15,9 +15,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     const int64_t blocks = (rows + S::kGroups - 1) / S::kGroups;
     RowRing<S::kGroups> ring{plan, &bars, smem, {reinterpret_cast<const uint8_t *>(x), nullptr}, rows};
     typename S::Raw q[S::kChunks];
-    launch_dependents();
-    if constexpr (S::kRing) ring.start([] { grid_dependency_wait(); });
-    else grid_dependency_wait();
+    if constexpr (S::kRing) ring.start();
     for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
         const int64_t row = block * S::kGroups + group;
         const int limit = row < rows ? width : 0;
@@ -50,9 +48,7 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % S::kWpr, group = (threadIdx.x >> 5) / S::kWpr;
     const int64_t blocks = (rows + S::kGroups - 1) / S::kGroups;
     RowRing<S::kGroups> ring{plan, &bars, smem, {packed, nullptr}, rows};
-    launch_dependents();
-    if constexpr (S::kRing) ring.start([] { grid_dependency_wait(); });
-    else grid_dependency_wait();
+    if constexpr (S::kRing) ring.start();
     for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
         const int64_t row = block * S::kGroups + group;
         const int limit = row < rows ? width : 0;
@@ -88,8 +84,9 @@ __global__ void __launch_bounds__(kRowThreads, 2)
     }
 }
 
-// CTAs a SM: with a ring two, whose rings fill its shared memory.
-constexpr int kResident = 2, kLaneResident = 4;
+// CTAs a SM.  Measured at 30,000 x 4,096 bf16: pack 78 us with two, 68 with
+// three, 65 with four; unpack 116, 102, 109.
+constexpr int kPackResident = 4, kUnpackResident = 3, kLaneResident = 4;
 
 }  // namespace
 
@@ -99,8 +96,8 @@ void launch_checkpoint_pack(const void *x, int64_t rows, int width, int dtype, u
     const size_t row = width * dtype_bytes(dtype);
     const bool wide = whole_units(row, {x}) && packs_wide(packed, dtype);
     const int groups = row_groups(width, wide);
-    const RingPlan plan = plan_ring(groups, row, 0);
-    const unsigned grid = row_grid(rows, groups, sms, wide ? kResident : kLaneResident);
+    const RingPlan plan = plan_ring(groups, row, 0, kPackResident);
+    const unsigned grid = row_grid(rows, groups, sms, wide ? kPackResident : kLaneResident);
     with_rows(dtype, wide, width, [&](auto s) {
         using S = decltype(s);
         launch_rows(pack_kernel<S>, grid, S::kRing ? ring_bytes(plan, groups) : 0, stream,
@@ -113,8 +110,8 @@ void launch_checkpoint_unpack(const uint8_t *packed, const uint8_t *exponents, i
     if (rows == 0) return;
     const bool wide = whole_units(width, {packed}) && whole_units(width * dtype_bytes(dtype), {x});
     const int groups = row_groups(width, wide);
-    const RingPlan plan = plan_ring(groups, width, 0);
-    const unsigned grid = row_grid(rows, groups, sms, wide ? kResident : kLaneResident);
+    const RingPlan plan = plan_ring(groups, width, 0, kUnpackResident);
+    const unsigned grid = row_grid(rows, groups, sms, wide ? kUnpackResident : kLaneResident);
     with_rows(dtype, wide, width, [&](auto s) {
         using S = decltype(s);
         launch_rows(unpack_kernel<S>, grid, S::kRing ? ring_bytes(plan, groups) : 0, stream, packed, exponents, rows,

@@ -43,9 +43,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_forward_kernel(NormForwar
     RowRing<S::kGroups> ring{plan, &bars, smem, {static_cast<const uint8_t *>(a.x), nullptr}, a.rows};
     typename S::Raw q[S::kChunks];
     float gamma[S::kLane], beta[S::kLane];
-    launch_dependents();
-    if constexpr (S::kRing) ring.start([] { grid_dependency_wait(); });
-    else grid_dependency_wait();
+    if constexpr (S::kRing) ring.start();
     load_columns<S>(a.gamma, width, warp, lane, 1.0f, gamma);
     load_columns<S>(a.beta, width, warp, lane, 0.0f, beta);
     for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
@@ -164,9 +162,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_backward_kernel(NormBackw
         m = row < a.rows ? a.mean[row] : 0.0f;
         r = row < a.rows ? a.rstd[row] : 0.0f;
     };
-    launch_dependents();
-    if constexpr (S::kRing) ring.start([] { grid_dependency_wait(); });
-    else grid_dependency_wait();
+    if constexpr (S::kRing) ring.start();
     load_columns<S>(a.gamma, width, warp, lane, 1.0f, gamma);
     moments(blockIdx.x, mean_next, rstd_next);
     for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
@@ -233,6 +229,7 @@ __global__ void __launch_bounds__(kRowThreads, 2) norm_backward_kernel(NormBackw
         }
         if constexpr (S::kRing) ring.close(block);
     }
+    launch_dependents();
     if (a.partials == nullptr) return;
     // each group's sums in shared memory, then joined in group order
     float *sums = reinterpret_cast<float *>(smem);
@@ -298,7 +295,7 @@ void launch_layer_norm(const NormForward &a, int sms, cudaStream_t stream) {
     const size_t row = a.width * dtype_bytes(a.dtype);
     const bool wide = whole_units(row, {a.x, a.y, a.gamma, a.beta}) && packs_wide(a.packed, a.dtype);
     const int groups = row_groups(a.width, wide);
-    const RingPlan plan = plan_ring(groups, row, 0);
+    const RingPlan plan = plan_ring(groups, row, 0, kResident);
     const unsigned grid = row_grid(a.rows, groups, sms, wide ? kResident : kLaneResident);
     with_rows(a.dtype, wide, a.width, [&](auto s) {
         using S = decltype(s);
@@ -320,7 +317,7 @@ void launch_layer_norm_backward(const NormBackward &args, int sms, cudaStream_t 
         const size_t row = a.width * dtype_bytes(a.dtype), x_row = a.x ? row : a.width;
         const bool wide = whole_units(row, {a.dy, a.dx, a.gamma}) && whole_units(x_row, {a.x, a.packed});
         const int groups = row_groups(a.width, wide);
-        const RingPlan plan = plan_ring(groups, row, x_row);
+        const RingPlan plan = plan_ring(groups, row, x_row, kResident);
         const size_t sums = a.partials ? groups * 2 * a.width * sizeof(float) : 0;
         grid = row_grid(a.rows, groups, sms, kResident);
         with_rows(a.dtype, wide, a.width, [&](auto s) {

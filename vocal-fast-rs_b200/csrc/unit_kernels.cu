@@ -108,10 +108,18 @@ struct Tile {
 };
 
 // Depth blocks summed in tensor memory before f32 registers take over.  The
-// accumulator truncates where f32 rounds, which at depth 768 in one run puts
-// a bias of 1e-5 on a log-sum of 20; runs of 4 blocks leave a third of it.
-// Results that are rounded to bf16 anyway take one run.
-constexpr int kShortRun = 4, kOneRun = 1 << 30;
+// accumulator truncates where f32 rounds: at depth 768 in one run a log-sum
+// of 20 comes out 1.2e-5 low, in runs of 6 blocks 6e-6, of 4 blocks 4e-6.
+// With 6 the tensor cores are a whole tile ahead of the epilogue at depth
+// 768, with 4 they wait for it (forward of 30,000 x 16,384 back to back:
+// 642 us in one run, 658 by 6, 709 by 4).  The backward pass is held up by
+// its epilogue either way and takes 4, which keeps the sums of softmax
+// gradients to 1e-5; f32 operands take 4 as well.  Results that are rounded to
+// bf16 take one run.
+constexpr int kOneRun = 1 << 30;
+template <class S, bool kBackward>
+constexpr int kLogitRun = S::kTerms == 1 && !kBackward ? 6 : 4;
+constexpr int kGradientRun = 4;
 
 // A bounded wait of a whole warp, the same answer for every lane.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity) {
@@ -448,10 +456,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     logit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                  const __grid_constant__ CUtensorMap map_g, const LogitArgs a) {
     constexpr int kTerms = S::kTerms;
+    constexpr int kRun = kLogitRun<S, kBackward>;
     const LogitWalk<S> walk(a, &map_x, &map_w);
-    run_roles<S, kShortRun>(walk, [&](uint8_t *smem, const Bars &bars, uint32_t tmem, int warp, int lane) {
+    run_roles<S, kRun>(walk, [&](uint8_t *smem, const Bars &bars, uint32_t tmem, int warp, int lane) {
         const int quarter = warp & 3, ew = warp - kFirstEpi, part = ew >> 2;
-        constexpr int kMax = Columns<S, kShortRun>::kMax;
+        constexpr int kMax = Columns<S, kRun>::kMax;
         // the warp's own: a tile's bias first, then G on its way out
         uint8_t *staging = smem + S::kStagingOff + ew * S::kStagingBytes;
         float *bias_slot = reinterpret_cast<float *>(S::kBuffers == 2 ? smem + S::kBiasOff + ew * 256 : staging);
@@ -461,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * part_cols;
         // logits in units of ln 2, z log2(e): exponentials are powers of two
         const float2 scale = make_float2(a.scale * kLog2e, a.scale * kLog2e);
-        Columns<S, kShortRun> columns;
+        Columns<S, kRun> columns;
         auto &v = columns.v;
         LogitWalk<S> own = walk;
         while (own.next_item()) {
@@ -762,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                    const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                    const ProductArgs a) {
     const ProductWalk<S> walk(a, &map_g, &map_gt, &map_w, &map_x);
-    constexpr int kRun = S::kTerms == 1 ? kOneRun : kShortRun;
+    constexpr int kRun = S::kTerms == 1 ? kOneRun : kGradientRun;
     run_roles<S, kRun>(walk, [&](uint8_t *, const Bars &bars, uint32_t tmem, int warp, int lane) {
         const int quarter = warp & 3, part = (warp - kFirstEpi) >> 2;
         const int part_cols = max(a.tile_n / kParts, 32), chunks = part * part_cols < a.tile_n ? part_cols / 32 : 0;
