@@ -840,39 +840,59 @@ __global__ void __launch_bounds__(kThreads, 1)
     });
 }
 
-// out[i] = sum over the splits of part[s][i], in split order.
-template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const float *part, int64_t stride, int splits, int64_t count,
-                                                   T *out) {
-    launch_dependents();
-    grid_dependency_wait();
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < count;
-         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        float s = 0.0f;
-        for (int k = 0; k < splits; ++k) s += part[k * stride + i];
-        out[i] = from_f32<T>(s);
-    }
-}
+// What the products of a piece leave to do, in one launch: results whose
+// depth was split, out[i] = sum over the splits of part[s][i], and dbias, the
+// row blocks' column sums; each in order, the same bits every time.
+struct FinishArgs {
+    struct Join {
+        const float *part;
+        int64_t stride, count;
+        int splits;
+        unsigned blocks;  // CTAs, 0: nothing to join
+        void *out;
+    } join[2];
+    const float *sums;  // [parts][columns]
+    int64_t parts;
+    int32_t columns;
+    unsigned sum_blocks;  // CTAs of 32 columns, 0: no dbias
+    float *dbias;
+};
+constexpr int kFinishThreads = 1024;
 
-// dbias from the row tiles' column sums, in order: 32 columns a CTA, 32 warps over the rows.
-__global__ void __launch_bounds__(1024) dbias_kernel(const float *sums, int64_t parts, int32_t count, float *out) {
+template <typename T>
+__global__ void __launch_bounds__(kFinishThreads) finish_kernel(const FinishArgs a) {
     __shared__ float slots[32][33];
     launch_dependents();
     grid_dependency_wait();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int col = blockIdx.x * 32 + lane;
-    float s = 0.0f;
-    if (col < count) {
+    unsigned block = blockIdx.x;
+    if (block < a.sum_blocks) {
+        // 32 columns, 32 warps over the row blocks
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const int col = block * 32 + lane;
+        float s = 0.0f;
+        if (col < a.columns) {
 #pragma unroll 8
-        for (int64_t p = warp; p < parts; p += 32) s += sums[p * count + col];
-    }
-    slots[warp][lane] = s;
-    __syncthreads();
-    s = slots[lane][warp];  // column `warp` of the CTA, part `lane`
+            for (int64_t p = warp; p < a.parts; p += 32) s += a.sums[p * a.columns + col];
+        }
+        slots[warp][lane] = s;
+        __syncthreads();
+        s = slots[lane][warp];  // column `warp` of the CTA, part `lane`
 #pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-    const int c = blockIdx.x * 32 + warp;
-    if (lane == 0 && c < count) out[c] = s;
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+        const int c = block * 32 + warp;
+        if (lane == 0 && c < a.columns) a.dbias[c] = s;
+        return;
+    }
+    block -= a.sum_blocks;
+    const int which = block < a.join[0].blocks ? 0 : 1;
+    const auto &j = a.join[which];
+    if (which) block -= a.join[0].blocks;
+    for (int64_t i = static_cast<int64_t>(block) * kFinishThreads + threadIdx.x; i < j.count;
+         i += static_cast<int64_t>(j.blocks) * kFinishThreads) {
+        float s = 0.0f;
+        for (int k = 0; k < j.splits; ++k) s += j.part[k * j.stride + i];
+        static_cast<T *>(j.out)[i] = from_f32<T>(s);
+    }
 }
 
 // ---------------------------------------------------------------- operands
@@ -1314,21 +1334,21 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
             launch_groups<S>(product_kernel<S>, groups, stream, map_k_major(g, kTileM),
                              map_mn_major(g, kTileM), map_mn_major(w, p.tile_n), map_xt, q);
         }
-        auto join = [&](int i) {
-            const auto &o = q.one[i];
+        FinishArgs f{};
+        for (int i = 0; i < 2; ++i) {
+            // dx waits for the last piece
+            if (p.direct[i] || (i == 0 && first + count < a.k)) continue;
             const int64_t n = size[i] * a.width;
-            const int64_t blocks = std::min<int64_t>(ceil_div(n, 256), 16 * sms);
-            const int splits = i == 0 ? p.splits[0] : o.splits;
-            cuda_check(launch_pdl(join_kernel<T>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
-                                  static_cast<const float *>(o.part), o.part_stride, splits, n,
-                                  static_cast<T *>(o.out)));
-        };
-        if (!p.direct[1]) join(1);
-        if (!p.direct[0] && first + count == a.k) join(0);
-        if (a.dbias)
-            cuda_check(launch_pdl(dbias_kernel, dim3(static_cast<unsigned>(ceil_div(count, 32))), dim3(1024), 0,
-                                  stream, static_cast<const float *>(l.column_sums), ceil_div(a.rows, 32),
-                                  static_cast<int32_t>(count), a.dbias + first));
+            f.join[i] = {q.one[i].part, q.one[i].part_stride, n, i == 0 ? p.splits[0] : q.one[i].splits,
+                         static_cast<unsigned>(std::min<int64_t>(ceil_div(n, kFinishThreads), 4 * sms)), q.one[i].out};
+        }
+        if (a.dbias) {
+            f.sums = l.column_sums, f.parts = ceil_div(a.rows, 32), f.columns = static_cast<int32_t>(count);
+            f.sum_blocks = static_cast<unsigned>(ceil_div(count, 32)), f.dbias = a.dbias + first;
+        }
+        const unsigned blocks = f.sum_blocks + f.join[0].blocks + f.join[1].blocks;
+        if (blocks)
+            cuda_check(launch_pdl(finish_kernel<T>, dim3(blocks), dim3(kFinishThreads), 0, stream, f));
     }
 }
 
