@@ -1034,11 +1034,19 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 int terms_of(int dtype) { return dtype == kF32 ? 3 : 1; }
 
-// Columns of a tile: the widest that still gives every SM a tile.
+// Columns of a tile: the width whose rounds over the SMs are the shortest, a
+// tile costing its columns and some 32 for its start and its end.
 int tile_columns(int64_t m_tiles, int64_t cols, int terms, int sms) {
-    int n = terms == 1 ? 256 : 128;
-    while (n > 64 && m_tiles * ceil_div(cols, n) < sms) n /= 2;
-    return n;
+    int best = 0;
+    int64_t least = INT64_MAX;
+    for (int n = terms == 1 ? 256 : 128; n >= 64; n /= 2) {
+        const int64_t cost = ceil_div(m_tiles * ceil_div(cols, n), sms) * (n + 32);
+        if (cost < least) {
+            least = cost;
+            best = n;
+        }
+    }
+    return best;
 }
 
 // Whether CTA pairs serve a product of so many rows and columns: full tiles
