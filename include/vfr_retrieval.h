@@ -466,7 +466,8 @@ VFR_API int vfr_checkpoint_unpack(const uint8_t *packed, const uint8_t *exponent
  * outside [0, k) is none: loss 0, no gradient, whatever the frame holds.  A
  * unit whose bias is -inf takes no part and gets no gradient, whatever its
  * row holds (a label on it: loss +inf); when all are, lse is -inf.  With vfr_kmeans centroids c, a
- * bias of -scale |c|^2 / 2 gives the soft nearest-centroid choice.
+ * bias of -scale |c|^2 / 2 gives the soft nearest-centroid choice.  |scale|
+ * is 1e30 at most.
  * workspace: 256-byte aligned; f32 products are exact to 24 bits. */
 VFR_API int vfr_unit_loss(const void *x, const void *units, const float *bias, const int32_t *labels, int64_t rows,
                           int32_t k, int32_t width, int32_t dtype, float scale, float *loss, float *lse,

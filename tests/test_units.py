@@ -259,6 +259,8 @@ def test_layer_norm_backward_refusals(native, change, message):
     (dict(k=0), "unit count must be positive"),
     (dict(width=4097), "row width must be in 1..4096"),
     (dict(scale=float("inf")), "logit scale must be finite"),
+    (dict(scale=float("nan")), "logit scale must be finite"),
+    (dict(scale=-2e30), "logit scale must be finite"),
     (dict(units=None), "null unit loss binding"),
     (dict(labels=None), "null unit loss binding"),
     (dict(labels=ctypes.c_void_p(2)), "misaligned unit loss binding"),
@@ -447,6 +449,78 @@ def test_layer_norm_backward(cuda, rows, width, dtype, affine, align):
 
 
 @pytest.mark.gpu
+def test_layer_norm_unaligned_parameters(cuda):
+    """gamma, beta, dy or the checkpoint off a 16-byte boundary, each alone."""
+    from vfr import units as u
+
+    torch = cuda
+
+    def moved(t):
+        buf = torch.empty(t.numel() * t.element_size() + 4, dtype=torch.uint8, device="cuda")
+        out = buf[4:].view(t.dtype).view(t.shape)
+        out.copy_(t)
+        return out
+
+    x = _frames(torch, 77, 768, "f32", 5)
+    gamma, beta = torch.randn(768, device="cuda"), torch.randn(768, device="cuda")
+    dy = torch.randn(77, 768, device="cuda")
+    y, mean, rstd, saved = u.layer_norm(x, gamma, beta, checkpoint=True)
+    wy, _, _, n = ref_norm(x, gamma, beta, 1e-5)
+    size = x.double().abs().mean(1, keepdim=True) * rstd.double()[:, None]
+    tol = gamma.double().abs() * (64 * U * size + n.abs() * 80 * U) + 8 * U * (wy.abs() + beta.double().abs())
+    for g, b in ((moved(gamma), beta), (gamma, moved(beta))):
+        _within(u.layer_norm(x, g, b)[0], wy, tol + 64 * U * (64 * U * size) ** 2 + 2.0 ** -25)
+    other = u.Checkpoint(moved(saved.packed.view(torch.uint8)).view(torch.float8_e4m3fn), saved.exponents, saved.dtype)
+    assert torch.equal(u.checkpoint_unpack(other, torch.float32), u.checkpoint_unpack(saved, torch.float32))
+    for source in (x, saved, other):
+        values = x if source is x else u.checkpoint_unpack(saved, torch.float32)
+        wx, wg, wb, n, g = ref_norm_grad(dy, values, mean, rstd, gamma)
+        r = rstd.double()[:, None]
+        tol = 80 * U * r * (g.abs() + g.abs().mean(1, keepdim=True) + 2 * n.abs() * (g * n).abs().mean(1, keepdim=True)
+                            + n.abs().mean(1, keepdim=True) * g.abs()) + 2.0 ** -25
+        for d, gm in ((dy, gamma), (moved(dy), gamma), (dy, moved(gamma))):
+            dx, dgamma, dbeta = u.layer_norm_backward(d, source, mean, rstd, gm)
+            _within(dx, wx, tol + 2 * U * wx.abs())
+            _within(dgamma, wg, 100 * U * (dy.double().abs() * n.abs()).sum(0))
+            _within(dbeta, wb, 100 * U * dy.double().abs().sum(0))
+
+
+@pytest.mark.gpu
+def test_first_call_may_be_captured(cuda):
+    """A process whose first calls of the operators are inside a capture."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from vfr import units as u
+x = torch.randn(300, 256, device="cuda").bfloat16()
+w = torch.randn(400, 256, device="cuda").bfloat16()
+labels = torch.arange(300, dtype=torch.int32, device="cuda")
+dloss = torch.ones(300, device="cuda")
+def step():
+    y, mean, rstd, saved = u.layer_norm(x, checkpoint=True)
+    loss, lse = u.unit_loss(y, w, labels, 0.1)
+    dy, dw, _ = u.unit_loss_backward(y, w, labels, lse, dloss, 0.1)
+    return loss, dw, u.layer_norm_backward(dy, saved, mean, rstd)[0]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = step()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, step()))
+print("same")
+"""
+    from vfr import lib
+
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       env={**os.environ, "PYTHONPATH": lib.PKG})
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("width", [8, 129, 4096])
 def test_checkpoint_special_values(cuda, dtype, width):
@@ -593,6 +667,17 @@ def test_unit_loss_all_units_left_out_and_lowest_bias(cuda, dtype):
     gone = torch.where(low < -1e38, torch.full_like(low, -math.inf), low)
     want = u.unit_loss(x, w, labels, scale, gone)
     assert torch.equal(loss, want[0]) and torch.equal(lse, want[1])
+    # a label on such a unit: the loss is the bias's size (f32 holds no more of it)
+    on = torch.full_like(labels, 3)
+    loss, lse2 = u.unit_loss(x, w, on, scale, low)
+    assert torch.equal(lse2, lse) and torch.equal(loss, torch.full_like(loss, torch.finfo(torch.float32).max))
+    # every unit at the lowest: equal logits, as natural f32 logits would be
+    low[:] = torch.finfo(torch.float32).min
+    loss, lse = u.unit_loss(x, w, labels, scale, low)
+    valid = (labels >= 0) & (labels < 90)
+    assert torch.equal(lse, torch.full_like(lse, torch.finfo(torch.float32).min)) and not loss[valid].any()
+    dx, dw, db = u.unit_loss_backward(x, w, labels, lse, dloss, scale, low)
+    assert all(torch.isfinite(t).all() for t in (dx, dw, db))
 
 
 @pytest.mark.gpu

@@ -46,6 +46,13 @@ constexpr int kGroupM = 16;      // row tiles that share the units they read
 constexpr uint32_t kTmemCols = 512;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLowest = -3.402823466e38f;
+
+// A bias or log-sum in units of ln 2.  What lies below -2.36e38 (a mask by the
+// type's lowest value) stays finite, so that a row of such logits alone is a
+// softmax of equal ones, as it is in natural units.
+__device__ __forceinline__ float to_log2(float v) { return v == -INFINITY ? v : fmaxf(v * kLog2e, kLowest); }
+
 
 // 2^v by the hardware's approximation (2 units in the last place of f32 for
 // the arguments here, which are not above 0 but by rounding; results below
@@ -484,8 +491,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (kBackward) {
                 if (valid) {
                     // every unit left out (-inf): p = 0
-                    lse = a.lse[row] == -INFINITY ? 0.0f : a.lse[row] * kLog2e;
-                    grad = columns.bad ? NAN : a.dloss[row];
+                    lse = a.lse[row] == -INFINITY ? 0.0f : to_log2(a.lse[row]);
+                    grad = a.dloss[row];
                 }
             }
             for (int n = own.n; n < own.end; ++n) {
@@ -499,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int j = 0; j < kMax; ++j) {
                     const int c = col0 + 32 * j + lane;
                     const float b = c >= a.count ? -INFINITY : a.bias ? __ldg(a.bias + a.first + c) : 0.0f;
-                    bias_slot[32 * j + lane] = b * kLog2e;
+                    bias_slot[32 * j + lane] = to_log2(b);
                     out[j] = __ballot_sync(0xFFFFFFFFu, b == -INFINITY);
                 }
                 __syncwarp();
@@ -562,7 +569,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     sum = fmaf(sum, exp2_approx(top - from), s.x + s.y);
                     top = next;
                 } else {
-                    const float2 minus = make_float2(-lse, -lse), by = make_float2(grad, grad);
+                    const float scaled = columns.bad ? NAN : grad;
+                    const float2 minus = make_float2(-lse, -lse), by = make_float2(scaled, scaled);
 #pragma unroll
                     for (int j = 0; j < kMax; ++j) {
                         if (j >= chunks) break;
@@ -658,7 +666,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Joins the slots of each row: 32 rows a CTA, a warp for every eighth slot.
 __global__ void __launch_bounds__(256) loss_kernel(const float2 *partial, const float *target, const int32_t *labels,
-                                                   int64_t rows, int slots, int k, float *loss, float *lse) {
+                                                   const float *bias, int64_t rows, int slots, int k, float *loss,
+                                                   float *lse) {
     __shared__ float2 joined[8][32];
     launch_dependents();
     grid_dependency_wait();
@@ -681,13 +690,14 @@ __global__ void __launch_bounds__(256) loss_kernel(const float2 *partial, const 
 #pragma unroll
     for (int w = 1; w < 8; ++w) join(joined[w][lane]);
     const float l = top == -INFINITY && sum == 0.0f ? top : top + log2f(sum);
-    lse[row] = l * kLn2;
+    const float natural = l == kLowest ? kLowest : l * kLn2;  // see to_log2
+    lse[row] = natural;
     const int32_t t = labels[row];
     if (t < 0 || t >= k) {
         loss[row] = 0.0f;
     } else {
         const float z = target[row];
-        loss[row] = z == -INFINITY ? INFINITY : (l - z) * kLn2;
+        loss[row] = z == -INFINITY ? INFINITY : z == kLowest && l > kLowest ? natural - bias[t] : (l - z) * kLn2;
     }
 }
 
@@ -1264,7 +1274,7 @@ void forward(const UnitLoss &a, int sms, cudaStream_t stream) {
                      l);
     cuda_check(launch_pdl(loss_kernel, dim3(static_cast<unsigned>(ceil_div(a.rows, 32))), dim3(256), 0, stream,
                           static_cast<const float2 *>(l.partial), static_cast<const float *>(l.target), a.labels,
-                          a.rows, kParts * p.splits, static_cast<int>(a.k), a.loss, a.lse));
+                          a.bias, a.rows, kParts * p.splits, static_cast<int>(a.k), a.loss, a.lse));
 }
 
 template <typename T, int kTerms>

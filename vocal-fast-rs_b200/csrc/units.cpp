@@ -162,7 +162,7 @@ extern "C" int vfr_unit_loss(const void *x, const void *units, const float *bias
     return guarded(error, [&] {
         cudaStream_t s = vfr::given_stream(stream);
         vfr::check_units(rows, k, width, dtype);
-        require(std::isfinite(scale), "the logit scale must be finite");
+        require(std::fabs(scale) <= 1e30f, "the logit scale must be finite (1e30 at most)");
         if (rows == 0) return;
         require(x && units && labels && loss && lse, "null unit loss binding");
         require(vfr::aligned_to(vfr::dtype_bytes(dtype), {x, units}) &&
@@ -188,7 +188,7 @@ extern "C" int vfr_unit_loss_backward(const void *x, const void *units, const fl
     return guarded(error, [&] {
         cudaStream_t s = vfr::given_stream(stream);
         vfr::check_units(rows, k, width, dtype);
-        require(std::isfinite(scale), "the logit scale must be finite");
+        require(std::fabs(scale) <= 1e30f, "the logit scale must be finite (1e30 at most)");
         require(units && dunits && (rows == 0 || (x && labels && lse && dloss && dx)), "null unit loss binding");
         require(vfr::aligned_to(vfr::dtype_bytes(dtype), {x, units, dx, dunits}) &&
                     vfr::aligned_to(4, {bias, labels, lse, dloss, dbias}) && vfr::aligned_to(256, {workspace}),
