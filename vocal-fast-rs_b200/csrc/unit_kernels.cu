@@ -84,12 +84,14 @@ struct Shape {
     static constexpr uint32_t kABytes = 2 * kBoxBytes;
     static constexpr uint32_t kBBytes = kTileN / kCtas / 64 * kBoxBytes;
     static constexpr uint32_t kStageBytes = kTerms * (kABytes + kBBytes);
-    // G on its way out, per epilogue warp: 32 rows of 32 columns
-    static constexpr int kBuffers = kTerms == 1 && !kPair ? 2 : 1;
-    static constexpr uint32_t kStagingBytes = kBuffers * 32 * 32 * 2;
+    // Logits: per epilogue warp G on its way out, 32 rows of a part's columns,
+    // and a tile's bias (f32: in the same place, before G).
+    static constexpr uint32_t kStagingBytes = kPair ? 0 : 32 * kTileN / kParts * 2;
     static constexpr uint32_t kStagingOff = kStages * kStageBytes;
-    static constexpr uint32_t kBiasOff = kStagingOff + kEpiWarps * kStagingBytes;
-    static constexpr uint32_t kBarOff = kBiasOff + (kBuffers == 2 ? kEpiWarps * 256 : 0);
+    static constexpr bool kBiasApart = kTerms == 1 && !kPair;
+    static constexpr uint32_t kBiasBytes = kBiasApart ? 256 : kStagingBytes;
+    static constexpr uint32_t kBiasOff = kStagingOff + (kBiasApart ? kEpiWarps * kStagingBytes : 0);
+    static constexpr uint32_t kBarOff = kStagingOff + kEpiWarps * (kStagingBytes + (kBiasApart ? kBiasBytes : 0));
     static constexpr size_t kSmem = 1024 + kBarOff + 256;
     static_assert(kSmem <= 232448, "shared memory");
 };
@@ -278,37 +280,15 @@ __device__ __forceinline__ void multiply(uint8_t *smem, const Bars &bars, uint32
     }
 }
 
-// Epilogue warps: `load` leaves in v this lane's row of the warp's part of
-// the tile, 32 kMax columns.  The accumulator is free again as soon as it is in
-// registers.  Once a wait gave up (`bad`) v is not to be used, and every later
-// result is NaN, so that none of a call that went wrong looks like one.
-template <class S, int kRun>
-struct Columns {
-    static constexpr int kTerms = S::kTerms;
-    static constexpr int kMax = S::kTileN / kParts / 32;  // 32-column chunks of a part
-    float v[kMax][32];
+// Epilogue warps' side of the accumulators.  An accumulator is free again as
+// soon as it is in registers.  Once a wait gave up (`bad`) the registers are
+// not to be used, and every later result is NaN, so that none of a call that
+// went wrong looks like one.
+template <class S>
+struct Drain {
     uint32_t acc_count = 0;
     bool bad = false;
 
-    // All kMax chunks are read, those past a narrow tile's too: their columns
-    // exist and nobody uses them.
-    __device__ __forceinline__ void load(const Bars &bars, uint32_t base, int depth) {
-        uint32_t at = wait(bars, base);
-#pragma unroll
-        for (int j = 0; j < kMax; ++j) tc::tmem_ld32_nowait(at + 32 * j, v[j]);
-#pragma unroll
-        for (int j = 0; j < kMax; ++j) tc::tmem_wait_ld32(v[j]);
-        if constexpr (kTerms > 1) add_from(at + 128);
-        release(bars);
-        while (kRun != kOneRun && (depth -= kRun) > 0) {
-            at = wait(bars, base);
-            if constexpr (kTerms > 1) add_from(at + 128);
-            add_from(at);
-            release(bars);
-        }
-    }
-
-private:
     __device__ __forceinline__ uint32_t wait(const Bars &bars, uint32_t base) {
         if (!bad) bad = !warp_wait(&bars.acc_full[acc_count & 1], (acc_count >> 1) & 1);
         tc::tc_fence_after();
@@ -323,19 +303,94 @@ private:
         }
         ++acc_count;
     }
+    template <int kCount>
+    static __device__ __forceinline__ void add(float *a, const float (&b)[kCount]) {
+#pragma unroll
+        for (int i = 0; i < kCount; i += 2) {
+            const float2 s = add2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+            a[i] = s.x, a[i + 1] = s.y;
+        }
+    }
+};
+
+// `load` leaves in v this lane's row of the warp's part of the tile, 32 kMax
+// columns.  All are read, those past a narrow tile's too: they exist and
+// nobody uses them.
+template <class S, int kRun>
+struct Columns : Drain<S> {
+    static constexpr int kTerms = S::kTerms;
+    static constexpr int kMax = S::kTileN / kParts / 32;  // 32-column chunks of a part
+    float v[kMax][32];
+
+    __device__ __forceinline__ void load(const Bars &bars, uint32_t base, int depth) {
+        uint32_t at = this->wait(bars, base);
+#pragma unroll
+        for (int j = 0; j < kMax; ++j) tc::tmem_ld32_nowait(at + 32 * j, v[j]);
+#pragma unroll
+        for (int j = 0; j < kMax; ++j) tc::tmem_wait_ld32(v[j]);
+        if constexpr (kTerms > 1) add_from(at + 128);
+        this->release(bars);
+        while (kRun != kOneRun && (depth -= kRun) > 0) {
+            at = this->wait(bars, base);
+            if constexpr (kTerms > 1) add_from(at + 128);
+            add_from(at);
+            this->release(bars);
+        }
+    }
+
+private:
     __device__ __forceinline__ void add_from(uint32_t at) {
 #pragma unroll
         for (int j = 0; j < 2 * kMax; ++j) {
             float u[16];
             tc::tmem_ld16_nowait(at + 16 * j, u);
             tc::tmem_wait_ld(u);
-            float *w = v[j / 2] + 16 * (j & 1);
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float2 s = add2(make_float2(w[i], w[i + 1]), make_float2(u[i], u[i + 1]));
-                w[i] = s.x, w[i + 1] = s.y;
-            }
+            this->add(v[j / 2] + 16 * (j & 1), u);
         }
+    }
+};
+
+// The same part of the tile as a matrix product's accumulators lie: lane l
+// holds, for q < 4, row 16 (q / 2) + 8 (q % 2) + l / 4, and of it columns
+// 8 i + 2 (l % 4) and + 1 for i < 4 kMax.  A row's column sums then take 8 lanes
+// and not 32, and 8 x 8 tiles go to shared memory as they are.
+template <class S, int kRun>
+struct Fragments : Drain<S> {
+    static constexpr int kTerms = S::kTerms;
+    static constexpr int kMax = S::kTileN / kParts / 32;
+    static constexpr int kBlocks = 4 * kMax;  // of 8 columns
+    float v[2][4 * kBlocks];  // [q / 2][4 i + 2 (q % 2) + e]
+
+    __device__ __forceinline__ float &at(int q, int i, int e) { return v[q >> 1][4 * i + 2 * (q & 1) + e]; }
+    __device__ __forceinline__ float2 pair(int q, int i) {
+        return make_float2(at(q, i, 0), at(q, i, 1));
+    }
+    __device__ __forceinline__ void set(int q, int i, float2 p) { at(q, i, 0) = p.x, at(q, i, 1) = p.y; }
+
+    __device__ __forceinline__ void load(const Bars &bars, uint32_t base, int depth) {
+        uint32_t from = this->wait(bars, base);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) tc::tmem_take_rows(from + (static_cast<uint32_t>(16 * h) << 16), v[h]);
+        if constexpr (kTerms > 1) add_from(from + 128);
+        this->release(bars);
+        while ((depth -= kRun) > 0) {
+            from = this->wait(bars, base);
+            if constexpr (kTerms > 1) add_from(from + 128);
+            add_from(from);
+            this->release(bars);
+        }
+    }
+
+private:
+    __device__ __forceinline__ void add_from(uint32_t from) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < kMax; ++j) {
+                float u[16];
+                tc::tmem_take_rows(from + (static_cast<uint32_t>(16 * h) << 16) + 32 * j, u);
+                this->add(v[h] + 16 * j, u);
+            }
     }
 };
 
@@ -458,210 +513,258 @@ struct LogitWalk {
     }
 };
 
+// The warp's place in the tile: TMEM lane quarter and part of the columns.  A
+// tile of 64 columns occupies two parts of 32.
+struct Place {
+    int quarter, part, part_cols, chunks;
+    uint32_t base;
+    __device__ __forceinline__ Place(uint32_t tmem, int warp, int tile_n)
+        : quarter(warp & 3), part((warp - kFirstEpi) >> 2), part_cols(max(tile_n / kParts, 32)),
+          chunks(part * part_cols < tile_n ? part_cols / 32 : 0),
+          base(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * part_cols) {}
+};
+
+// Forward: per row and item the running (maximum, sum), a row to a lane.
+template <class S>
+__device__ __forceinline__ void fold_logits(const LogitArgs &a, LogitWalk<S> own, uint8_t *smem, const Bars &bars,
+                                            uint32_t tmem, int warp, int lane) {
+    constexpr int kRun = kLogitRun<S, false>;
+    const Place at(tmem, warp, a.tile_n);
+    constexpr int kMax = Columns<S, kRun>::kMax;
+    float *bias_slot = reinterpret_cast<float *>(smem + S::kBiasOff + (warp - kFirstEpi) * S::kBiasBytes);
+    // logits in units of ln 2, z log2(e): exponentials are powers of two
+    const float2 scale = make_float2(a.scale * kLog2e, a.scale * kLog2e);
+    Columns<S, kRun> columns;
+    auto &v = columns.v;
+    while (own.next_item()) {
+        const int64_t row = static_cast<int64_t>(own.block()) * kTileM + at.quarter * 32 + lane;
+        const bool live = row < a.rows;
+        int32_t label = live ? a.labels[row] : -1;
+        if (label >= a.k) label = -1;
+        float top = -INFINITY, sum = 0.0f;
+        for (int n = own.n; n < own.end; ++n) {
+            const int col0 = n * a.tile_n + at.part * at.part_cols;
+            // bias of the part's columns, and which take no part: units left
+            // out and columns past the last, -inf whatever the product is
+            uint32_t out[kMax];
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < kMax; ++j) {
+                const int c = col0 + 32 * j + lane;
+                const float b = c >= a.count ? -INFINITY : a.bias ? __ldg(a.bias + c) : 0.0f;
+                bias_slot[32 * j + lane] = to_log2(b);
+                out[j] = __ballot_sync(0xFFFFFFFFu, b == -INFINITY);
+            }
+            __syncwarp();
+            columns.load(bars, at.base, a.k_blocks);
+#pragma unroll
+            for (int j = 0; j < kMax; ++j) {
+                if (j >= at.chunks) break;
+                const float4 *b4 = reinterpret_cast<const float4 *>(bias_slot + 32 * j);
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    const float4 b = b4[i / 4];
+                    const float2 lo = fma2(make_float2(v[j][i], v[j][i + 1]), scale, make_float2(b.x, b.y));
+                    const float2 hi = fma2(make_float2(v[j][i + 2], v[j][i + 3]), scale, make_float2(b.z, b.w));
+                    v[j][i] = lo.x, v[j][i + 1] = lo.y, v[j][i + 2] = hi.x, v[j][i + 3] = hi.y;
+                }
+                if (out[j]) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (out[j] >> i & 1) v[j][i] = -INFINITY;
+                }
+            }
+            const int hit = label - col0;  // the label's column in the part
+            if (label >= 0 && hit >= 0 && hit < 32 * at.chunks) {
+#pragma unroll
+                for (int j = 0; j < kMax; ++j)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (32 * j + i == hit) a.target[row] = v[j][i];
+            }
+            float m8[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m8[i] = top;
+#pragma unroll
+            for (int j = 0; j < kMax; ++j) {
+                if (j >= at.chunks) break;
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) m8[i / 2 & 7] = fmaxf(m8[i / 2 & 7], fmaxf(v[j][i], v[j][i + 1]));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m8[i] = fmaxf(m8[i], m8[i + 4]);
+            const float next = fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3]));
+            const float from = next == -INFINITY ? 0.0f : next;
+            const float2 minus = make_float2(-from, -from);
+            float2 s4[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s4[i] = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < kMax; ++j) {
+                if (j >= at.chunks) break;
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 d = add2(make_float2(v[j][i], v[j][i + 1]), minus);
+                    s4[i / 2 & 3] = add2(s4[i / 2 & 3], make_float2(exp2_approx(d.x), exp2_approx(d.y)));
+                }
+            }
+            const float2 s = add2(add2(s4[0], s4[1]), add2(s4[2], s4[3]));
+            sum = fmaf(sum, exp2_approx(top - from), s.x + s.y);
+            top = next;
+        }
+        if (columns.bad) sum = NAN;
+        if (live) a.partial[(own.n / a.span * kParts + at.part) * a.rows + row] = make_float2(top, sum);
+    }
+}
+
+// Backward: G in bf16 (f32: three terms) to global memory, and its column sums.
+template <class S>
+__device__ __forceinline__ void store_gradients(const LogitArgs &a, const CUtensorMap *map_g, LogitWalk<S> own,
+                                                uint8_t *smem, const Bars &bars, uint32_t tmem, int warp, int lane) {
+    constexpr int kTerms = S::kTerms, kRun = kLogitRun<S, true>;
+    const Place at(tmem, warp, a.tile_n);
+    using Frag = Fragments<S, kRun>;
+    constexpr int kMax = Frag::kMax, kBlocks = Frag::kBlocks;
+    float *bias_slot = reinterpret_cast<float *>(smem + S::kBiasOff + (warp - kFirstEpi) * S::kBiasBytes);
+    uint8_t *staging = smem + S::kStagingOff + (warp - kFirstEpi) * S::kStagingBytes;
+    const float2 scale = make_float2(a.scale * kLog2e, a.scale * kLog2e);
+    const int pair = 2 * (lane & 3);  // the lane's first column of each 8
+    Frag f;
+    while (own.next_item()) {
+        const int64_t row0 = static_cast<int64_t>(own.block()) * kTileM + at.quarter * 32;
+        int32_t label[4];
+        float lse[4], grad[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int64_t row = row0 + 16 * (q >> 1) + 8 * (q & 1) + (lane >> 2);
+            label[q] = row < a.rows ? a.labels[row] : -1;
+            const bool valid = label[q] >= 0 && label[q] < a.k;
+            if (!valid) label[q] = -1;
+            // Without a label p = 2^-inf and G = 0 (its frame is a row of
+            // zeros); with every unit left out p = 2^(-inf - 0)
+            lse[q] = !valid ? INFINITY : a.lse[row] == -INFINITY ? 0.0f : to_log2(a.lse[row]);
+            grad[q] = valid ? a.dloss[row] : 0.0f;
+        }
+        for (int n = own.n; n < own.end; ++n) {
+            const int col0 = n * a.tile_n + at.part * at.part_cols;  // within the launch's units
+            // -inf for units left out (rows of zeros) and columns past the last
+            if (!S::kBiasApart) tc::bulk_wait_read<0>();
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < kMax; ++j) {
+                const int c = col0 + 32 * j + lane;
+                bias_slot[32 * j + lane] =
+                    c >= a.count ? -INFINITY : a.bias ? to_log2(__ldg(a.bias + a.first + c)) : 0.0f;
+            }
+            __syncwarp();
+            f.load(bars, at.base, a.k_blocks);
+#pragma unroll
+            for (int i = 0; i < kBlocks; ++i) {
+                if (i >= 4 * at.chunks) break;
+                const float2 b = *reinterpret_cast<const float2 *>(bias_slot + 8 * i + pair);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float2 d = add2(fma2(f.pair(q, i), scale, b), make_float2(-lse[q], -lse[q]));
+                    f.set(q, i, make_float2(exp2_approx(d.x), exp2_approx(d.y)));
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                // the label's column, where the unit takes part
+                const int hit = label[q] - a.first - col0;
+                if (label[q] >= 0 && hit >= 0 && hit < 32 * at.chunks && (hit & 6) == pair &&
+                    bias_slot[hit] != -INFINITY) {
+#pragma unroll
+                    for (int i = 0; i < kBlocks; ++i)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (8 * i + e + pair == hit) f.at(q, i, e) -= 1.0f;
+                }
+                const float by = f.bad ? NAN : grad[q];
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i) f.set(q, i, mul2(f.pair(q, i), make_float2(by, by)));
+            }
+            if (a.column_sums) {
+                // the lane's four rows, then the eight lanes of a column: lane
+                // group l / 4 ends with block l / 4 (of 32 columns: l / 4 % 4)
+                float2 s[kBlocks];
+#pragma unroll
+                for (int i = 0; i < kBlocks; ++i)
+                    s[i] = add2(add2(f.pair(0, i), f.pair(1, i)), add2(f.pair(2, i), f.pair(3, i)));
+#pragma unroll
+                for (int o = kBlocks / 2; o; o >>= 1) {
+                    const bool upper = lane & (4 * o);
+#pragma unroll
+                    for (int i = 0; i < o; ++i) {
+                        const float2 keep = upper ? s[i + o] : s[i], send = upper ? s[i] : s[i + o];
+                        s[i] = add2(keep, make_float2(__shfl_xor_sync(0xFFFFFFFFu, send.x, 4 * o),
+                                                      __shfl_xor_sync(0xFFFFFFFFu, send.y, 4 * o)));
+                    }
+                }
+                if constexpr (kBlocks == 4)
+                    s[0] = add2(s[0], make_float2(__shfl_xor_sync(0xFFFFFFFFu, s[0].x, 16),
+                                                  __shfl_xor_sync(0xFFFFFFFFu, s[0].y, 16)));
+                const int block = lane >> 2, c = col0 + 8 * block + pair;
+                if (block < 4 * at.chunks) {
+                    float *sums = a.column_sums + row0 / 32 * a.count;
+                    if (c < a.count) sums[c] = s[0].x;
+                    if (c + 1 < a.count) sums[c + 1] = s[0].y;
+                }
+            }
+            // a factor of its own products, rounded as any operand of theirs;
+            // a store takes the part's 64 columns at once, or 32 of a narrow part
+            const int units = 4 * at.chunks;  // of 16 bytes in a row of a store
+#pragma unroll
+            for (int p = 0; p < kTerms; ++p) {
+                if (at.chunks == 0) break;
+                tc::bulk_wait_read<0>();
+                __syncwarp();
+                // swizzled as SWIZZLE_128B or SWIZZLE_64B expects; tile l / 8
+                // of four: rows + 8 (tile % 2), units + tile / 2
+                const int r = lane & 15, turn = kMax == 2 && units == 8 ? r & 7 : r >> 1 & 3;
+                const uint32_t to = tc::smem_u32(staging) + r * 16 * units;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < kBlocks; i += 2) {
+                        if (i >= units) break;
+                        uint32_t w[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int q = 2 * h + (e & 1), block = i + (e >> 1);
+                            const float2 x = f.pair(q, block);
+                            const __nv_bfloat162 y = __floats2bfloat162_rn(x.x, x.y);
+                            w[e] = *reinterpret_cast<const uint32_t *>(&y);
+                            if (p + 1 < kTerms) {
+                                const float2 z = __bfloat1622float2(y);
+                                f.set(q, block, make_float2(x.x - z.x, x.y - z.y));
+                            }
+                        }
+                        tc::store_tiles(to + 256 * units * h + (((i + (lane >> 4)) ^ turn) << 4), w[0], w[1], w[2],
+                                        w[3]);
+                    }
+                tc::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0 && col0 < a.count && row0 < a.rows)
+                    tc::tma_store_3d(map_g, staging, col0, static_cast<int32_t>(row0), p);
+                if (lane == 0) tc::bulk_commit();
+            }
+        }
+    }
+    if (lane == 0) tc::bulk_wait_all();
+    __syncwarp();
+}
+
 template <class S, bool kBackward>
 __global__ void __launch_bounds__(kThreads, 1)
     logit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                  const __grid_constant__ CUtensorMap map_g, const LogitArgs a) {
-    constexpr int kTerms = S::kTerms;
-    constexpr int kRun = kLogitRun<S, kBackward>;
     const LogitWalk<S> walk(a, &map_x, &map_w);
-    run_roles<S, kRun>(walk, [&](uint8_t *smem, const Bars &bars, uint32_t tmem, int warp, int lane) {
-        const int quarter = warp & 3, ew = warp - kFirstEpi, part = ew >> 2;
-        constexpr int kMax = Columns<S, kRun>::kMax;
-        // the warp's own: a tile's bias first, then G on its way out
-        uint8_t *staging = smem + S::kStagingOff + ew * S::kStagingBytes;
-        float *bias_slot = reinterpret_cast<float *>(S::kBuffers == 2 ? smem + S::kBiasOff + ew * 256 : staging);
-        uint32_t stores = 0;
-        // a tile of 64 columns occupies two parts of 32
-        const int part_cols = max(a.tile_n / kParts, 32), chunks = part * part_cols < a.tile_n ? part_cols / 32 : 0;
-        const uint32_t base = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * part_cols;
-        // logits in units of ln 2, z log2(e): exponentials are powers of two
-        const float2 scale = make_float2(a.scale * kLog2e, a.scale * kLog2e);
-        Columns<S, kRun> columns;
-        auto &v = columns.v;
-        LogitWalk<S> own = walk;
-        while (own.next_item()) {
-            const int64_t row0 = static_cast<int64_t>(own.block()) * kTileM + quarter * 32, row = row0 + lane;
-            const bool live = row < a.rows;
-            int32_t label = live ? a.labels[row] : -1;
-            if (label >= a.k) label = -1;
-            const bool valid = label >= 0;
-            float top = -INFINITY, sum = 0.0f;  // forward
-            float lse = 0.0f, grad = 0.0f;      // backward
-            if constexpr (kBackward) {
-                if (valid) {
-                    // every unit left out (-inf): p = 0
-                    lse = a.lse[row] == -INFINITY ? 0.0f : to_log2(a.lse[row]);
-                    grad = a.dloss[row];
-                }
-            }
-            for (int n = own.n; n < own.end; ++n) {
-                const int col0 = n * a.tile_n + part * part_cols;  // within the launch's units
-                // bias of the part's columns, and which take no part: units
-                // left out and columns past the last
-                uint32_t out[kMax];
-                if constexpr (kBackward && S::kBuffers == 1) tc::bulk_wait_read<0>();
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < kMax; ++j) {
-                    const int c = col0 + 32 * j + lane;
-                    const float b = c >= a.count ? -INFINITY : a.bias ? __ldg(a.bias + a.first + c) : 0.0f;
-                    bias_slot[32 * j + lane] = to_log2(b);
-                    out[j] = __ballot_sync(0xFFFFFFFFu, b == -INFINITY);
-                }
-                __syncwarp();
-                columns.load(bars, base, a.k_blocks);
-#pragma unroll
-                for (int j = 0; j < kMax; ++j) {
-                    if (j >= chunks) break;
-                    const float4 *b4 = reinterpret_cast<const float4 *>(bias_slot + 32 * j);
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
-                        const float4 b = b4[i / 4];
-                        const float2 lo = fma2(make_float2(v[j][i], v[j][i + 1]), scale, make_float2(b.x, b.y));
-                        const float2 hi = fma2(make_float2(v[j][i + 2], v[j][i + 3]), scale, make_float2(b.z, b.w));
-                        v[j][i] = lo.x, v[j][i + 1] = lo.y, v[j][i + 2] = hi.x, v[j][i + 3] = hi.y;
-                    }
-                    // -inf whatever the product is (backward: rows of zeros)
-                    if (!kBackward && out[j]) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (out[j] >> i & 1) v[j][i] = -INFINITY;
-                    }
-                }
-                if constexpr (!kBackward) {
-                    const int hit = label - a.first - col0;  // the label's column in the part
-                    if (valid && hit >= 0 && hit < 32 * chunks) {
-#pragma unroll
-                        for (int j = 0; j < kMax; ++j)
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (32 * j + i == hit) a.target[row] = v[j][i];
-                    }
-                    float m8[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) m8[i] = top;
-#pragma unroll
-                    for (int j = 0; j < kMax; ++j) {
-                        if (j >= chunks) break;
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2)
-                            m8[i / 2 & 7] = fmaxf(m8[i / 2 & 7], fmaxf(v[j][i], v[j][i + 1]));
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) m8[i] = fmaxf(m8[i], m8[i + 4]);
-                    const float next = fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3]));
-                    const float from = next == -INFINITY ? 0.0f : next;
-                    const float2 minus = make_float2(-from, -from);
-                    float2 s4[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s4[i] = make_float2(0.0f, 0.0f);
-#pragma unroll
-                    for (int j = 0; j < kMax; ++j) {
-                        if (j >= chunks) break;
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float2 d = add2(make_float2(v[j][i], v[j][i + 1]), minus);
-                            s4[i / 2 & 3] = add2(s4[i / 2 & 3], make_float2(exp2_approx(d.x), exp2_approx(d.y)));
-                        }
-                    }
-                    const float2 s = add2(add2(s4[0], s4[1]), add2(s4[2], s4[3]));
-                    sum = fmaf(sum, exp2_approx(top - from), s.x + s.y);
-                    top = next;
-                } else {
-                    const float scaled = columns.bad ? NAN : grad;
-                    const float2 minus = make_float2(-lse, -lse), by = make_float2(scaled, scaled);
-#pragma unroll
-                    for (int j = 0; j < kMax; ++j) {
-                        if (j >= chunks) break;
-                        const int col = col0 + 32 * j;
-                        const int hit = label - a.first - col;  // the label's column in the chunk
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float2 d = add2(make_float2(v[j][i], v[j][i + 1]), minus);
-                            v[j][i] = exp2_approx(d.x), v[j][i + 1] = exp2_approx(d.y);
-                        }
-                        if (valid && hit >= 0 && hit < 32 && !(out[j] >> hit & 1)) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i)
-                                if (i == hit) v[j][i] -= 1.0f;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float2 g = mul2(make_float2(v[j][i], v[j][i + 1]), by);
-                            v[j][i] = g.x, v[j][i + 1] = g.y;
-                        }
-                        if (!valid) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[j][i] = 0.0f;
-                        }
-                        if (a.column_sums) {
-                            // sums over the warp's 32 rows, 16 columns at a
-                            // time: lane i ends with column i & 15
-#pragma unroll
-                            for (int h = 0; h < 32; h += 16) {
-                                float s[16];
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) s[i] = v[j][h + i];
-#pragma unroll
-                                for (int o = 8; o; o >>= 1) {
-                                    const bool upper = lane & o;
-#pragma unroll
-                                    for (int i = 0; i < o; ++i) {
-                                        const float keep = upper ? s[i + o] : s[i];
-                                        s[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, upper ? s[i] : s[i + o], o);
-                                    }
-                                }
-                                s[0] += __shfl_xor_sync(0xFFFFFFFFu, s[0], 16);
-                                const int c = col + h + lane;
-                                if (lane < 16 && c < a.count)
-                                    a.column_sums[row0 / 32 * a.count + c] = s[0];
-                            }
-                        }
-                        // G in bf16 (f32: three terms): a factor of its own
-                        // products, rounded as any operand of theirs
-#pragma unroll
-                        for (int p = 0; p < kTerms; ++p) {
-                            tc::bulk_wait_read<S::kBuffers - 1>();
-                            __syncwarp();
-                            uint8_t *buf = staging + (S::kBuffers == 2 ? (stores++ & 1) * 2048 : 0);
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                uint32_t w[4];
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const int i = 8 * c + 2 * e;
-                                    const __nv_bfloat162 b = __floats2bfloat162_rn(v[j][i], v[j][i + 1]);
-                                    w[e] = *reinterpret_cast<const uint32_t *>(&b);
-                                    if (p + 1 < kTerms) {
-                                        const float2 f = __bfloat1622float2(b);
-                                        v[j][i] -= f.x;
-                                        v[j][i + 1] -= f.y;
-                                    }
-                                }
-                                // 64-byte rows, 16-byte units swizzled as SWIZZLE_64B expects
-                                *reinterpret_cast<uint4 *>(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)) =
-                                    make_uint4(w[0], w[1], w[2], w[3]);
-                            }
-                            tc::fence_proxy_async_smem();
-                            __syncwarp();
-                            if (lane == 0 && col < a.count && row0 < a.rows)
-                                tc::tma_store_3d(&map_g, buf, col, static_cast<int32_t>(row0), p);
-                            if (lane == 0) tc::bulk_commit();
-                        }
-                    }
-                }
-            }
-            if constexpr (!kBackward) {
-                if (columns.bad) sum = NAN;
-                if (live) a.partial[(own.n / a.span * kParts + part) * a.rows + row] = make_float2(top, sum);
-            }
-        }
-        if constexpr (kBackward) {
-            if (lane == 0) tc::bulk_wait_all();
-            __syncwarp();
-        }
-    });
+    run_roles<S, kLogitRun<S, kBackward>>(
+        walk, [&](uint8_t *smem, const Bars &bars, uint32_t tmem, int warp, int lane) {
+            if constexpr (kBackward) store_gradients<S>(a, &map_g, walk, smem, bars, tmem, warp, lane);
+            else fold_logits<S>(a, walk, smem, bars, tmem, warp, lane);
+        });
 }
 
 // Joins the slots of each row: 32 rows a CTA, a warp for every eighth slot.
@@ -1029,13 +1132,13 @@ CUtensorMap map_mn_major(const Terms &t, int cols) {
     const cuuint32_t box[4] = {64, kBlockK, static_cast<cuuint32_t>(cols / 64), 1};
     return encode(t, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-// G's stores: 32 by 32.
-CUtensorMap map_store(const Terms &t) {
+// G's stores: 32 rows by `cols` columns, 32 or 64.
+CUtensorMap map_store(const Terms &t, int cols) {
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(t.cols), static_cast<cuuint64_t>(t.rows),
                                 static_cast<cuuint64_t>(t.count)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(t.pitch) * 2, static_cast<cuuint64_t>(t.plane) * 2};
-    const cuuint32_t box[3] = {32, 32, 1};
-    return encode(t, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_64B);
+    const cuuint32_t box[3] = {static_cast<cuuint32_t>(cols), 32, 1};
+    return encode(t, 3, dims, strides, box, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // ---------------------------------------------------------------- plans
@@ -1307,7 +1410,7 @@ void backward(const UnitLoss &a, int sms, cudaStream_t stream) {
             using S = Shape<kTerms, false>;
             launch_groups<S>(logit_kernel<S, true>,
                              std::min<int64_t>(static_cast<int64_t>(l.m_tiles) * l.splits, sms), stream, map_x,
-                             map_k_major(w, l.tile_n), map_store(g), l);
+                             map_k_major(w, l.tile_n), map_store(g, l.tile_n == 256 ? 64 : 32), l);
         }
         ProductArgs q{};
         q.width = a.width, q.tile_n = p.tile_n;
