@@ -123,11 +123,11 @@ struct Tile {
 // 768, with 4 they wait for it (forward of 30,000 x 16,384 back to back:
 // 642 us in one run, 658 by 6, 709 by 4).  The backward pass is held up by
 // its epilogue either way and takes 4, which keeps the sums of softmax
-// gradients to 1e-5; f32 operands take 4 as well.  Results that are rounded to
-// bf16 take one run.
+// gradients to 1e-5.  f32 operands, six products a block, take 4 and 2 (2 in
+// the forward pass costs 6%).  Results that are rounded to bf16 take one run.
 constexpr int kOneRun = 1 << 30;
 template <class S, bool kBackward>
-constexpr int kLogitRun = S::kTerms == 1 && !kBackward ? 6 : 4;
+constexpr int kLogitRun = S::kTerms == 1 ? (kBackward ? 4 : 6) : (kBackward ? 2 : 4);
 constexpr int kGradientRun = 4;
 
 // A bounded wait of a whole warp, the same answer for every lane.
@@ -627,7 +627,9 @@ __device__ __forceinline__ void store_gradients(const LogitArgs &a, const CUtens
     constexpr int kMax = Frag::kMax, kBlocks = Frag::kBlocks;
     float *bias_slot = reinterpret_cast<float *>(smem + S::kBiasOff + (warp - kFirstEpi) * S::kBiasBytes);
     uint8_t *staging = smem + S::kStagingOff + (warp - kFirstEpi) * S::kStagingBytes;
-    const float2 scale = make_float2(a.scale * kLog2e, a.scale * kLog2e);
+    // natural units: where p nears 1 the difference of logit and log-sum is
+    // small, and scaling it afterwards loses nothing
+    const float2 scale = make_float2(a.scale, a.scale);
     const int pair = 2 * (lane & 3);  // the lane's first column of each 8
     Frag f;
     while (own.next_item()) {
@@ -640,9 +642,9 @@ __device__ __forceinline__ void store_gradients(const LogitArgs &a, const CUtens
             label[q] = row < a.rows ? a.labels[row] : -1;
             const bool valid = label[q] >= 0 && label[q] < a.k;
             if (!valid) label[q] = -1;
-            // Without a label p = 2^-inf and G = 0 (its frame is a row of
-            // zeros); with every unit left out p = 2^(-inf - 0)
-            lse[q] = !valid ? INFINITY : a.lse[row] == -INFINITY ? 0.0f : to_log2(a.lse[row]);
+            // Without a label p = exp(-inf) and G = 0 (its frame is a row of
+            // zeros); with every unit left out p = exp(-inf - 0)
+            lse[q] = !valid ? INFINITY : a.lse[row] == -INFINITY ? 0.0f : a.lse[row];
             grad[q] = valid ? a.dloss[row] : 0.0f;
         }
         for (int n = own.n; n < own.end; ++n) {
@@ -653,8 +655,7 @@ __device__ __forceinline__ void store_gradients(const LogitArgs &a, const CUtens
 #pragma unroll
             for (int j = 0; j < kMax; ++j) {
                 const int c = col0 + 32 * j + lane;
-                bias_slot[32 * j + lane] =
-                    c >= a.count ? -INFINITY : a.bias ? to_log2(__ldg(a.bias + a.first + c)) : 0.0f;
+                bias_slot[32 * j + lane] = c >= a.count ? -INFINITY : a.bias ? __ldg(a.bias + a.first + c) : 0.0f;
             }
             __syncwarp();
             f.load(bars, at.base, a.k_blocks);
@@ -665,7 +666,8 @@ __device__ __forceinline__ void store_gradients(const LogitArgs &a, const CUtens
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const float2 d = add2(fma2(f.pair(q, i), scale, b), make_float2(-lse[q], -lse[q]));
-                    f.set(q, i, make_float2(exp2_approx(d.x), exp2_approx(d.y)));
+                    const float2 e = mul2(d, make_float2(kLog2e, kLog2e));
+                    f.set(q, i, make_float2(exp2_approx(e.x), exp2_approx(e.y)));
                 }
             }
 #pragma unroll
