@@ -524,6 +524,17 @@ struct Place {
           base(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + part * part_cols) {}
 };
 
+// The lane's biases of a part that starts at column `at` - lane of the
+// launch's units, -inf past the last.
+template <int kMax>
+__device__ __forceinline__ void column_bias(const LogitArgs &a, int at, float (&bias)[kMax]) {
+#pragma unroll
+    for (int j = 0; j < kMax; ++j) {
+        const int c = at + 32 * j;
+        bias[j] = c >= a.count ? -INFINITY : a.bias ? __ldg(a.bias + a.first + c) : 0.0f;
+    }
+}
+
 // Forward: per row and item the running (maximum, sum), a row to a lane.
 template <class S>
 __device__ __forceinline__ void fold_logits(const LogitArgs &a, LogitWalk<S> own, uint8_t *smem, const Bars &bars,
@@ -542,21 +553,22 @@ __device__ __forceinline__ void fold_logits(const LogitArgs &a, LogitWalk<S> own
         int32_t label = live ? a.labels[row] : -1;
         if (label >= a.k) label = -1;
         float top = -INFINITY, sum = 0.0f;
+        float bias[kMax];
+        column_bias(a, own.n * a.tile_n + at.part * at.part_cols + lane, bias);
         for (int n = own.n; n < own.end; ++n) {
             const int col0 = n * a.tile_n + at.part * at.part_cols;
-            // bias of the part's columns, and which take no part: units left
-            // out and columns past the last, -inf whatever the product is
+            // which columns take no part: units left out and columns past the
+            // last, -inf whatever the product is
             uint32_t out[kMax];
             __syncwarp();
 #pragma unroll
             for (int j = 0; j < kMax; ++j) {
-                const int c = col0 + 32 * j + lane;
-                const float b = c >= a.count ? -INFINITY : a.bias ? __ldg(a.bias + c) : 0.0f;
-                bias_slot[32 * j + lane] = to_log2(b);
-                out[j] = __ballot_sync(0xFFFFFFFFu, b == -INFINITY);
+                bias_slot[32 * j + lane] = to_log2(bias[j]);
+                out[j] = __ballot_sync(0xFFFFFFFFu, bias[j] == -INFINITY);
             }
             __syncwarp();
             columns.load(bars, at.base, a.k_blocks);
+            column_bias(a, col0 + a.tile_n + lane, bias);  // the next tile's, while this one is worked on
 #pragma unroll
             for (int j = 0; j < kMax; ++j) {
                 if (j >= at.chunks) break;
@@ -647,18 +659,18 @@ __device__ __forceinline__ void store_gradients(const LogitArgs &a, const CUtens
             lse[q] = !valid ? INFINITY : a.lse[row] == -INFINITY ? 0.0f : a.lse[row];
             grad[q] = valid ? a.dloss[row] : 0.0f;
         }
+        float bias[kMax];
+        column_bias(a, own.n * a.tile_n + at.part * at.part_cols + lane, bias);
         for (int n = own.n; n < own.end; ++n) {
             const int col0 = n * a.tile_n + at.part * at.part_cols;  // within the launch's units
             // -inf for units left out (rows of zeros) and columns past the last
             if (!S::kBiasApart) tc::bulk_wait_read<0>();
             __syncwarp();
 #pragma unroll
-            for (int j = 0; j < kMax; ++j) {
-                const int c = col0 + 32 * j + lane;
-                bias_slot[32 * j + lane] = c >= a.count ? -INFINITY : a.bias ? __ldg(a.bias + a.first + c) : 0.0f;
-            }
+            for (int j = 0; j < kMax; ++j) bias_slot[32 * j + lane] = bias[j];
             __syncwarp();
             f.load(bars, at.base, a.k_blocks);
+            column_bias(a, col0 + a.tile_n + lane, bias);  // the next tile's, while this one is worked on
 #pragma unroll
             for (int i = 0; i < kBlocks; ++i) {
                 if (i >= 4 * at.chunks) break;
@@ -1171,12 +1183,13 @@ bool pairs_fit(int64_t rows, int64_t cols, int terms, int sms) {
     return terms == 1 && ceil_div(rows, 256) * ceil_div(cols, 256) >= sms && ceil_div(cols, 256) * 192 <= cols;
 }
 
-// Column tiles of an item: the fewest rounds of the grid, then the fewest items.
+// Column tiles of an item: the shortest rounds of the grid, an item costing a
+// quarter of a tile for its start.
 int item_span(int64_t m_tiles, int64_t n_tiles, int sms) {
     int64_t best = INT64_MAX, span = 1;
     for (int64_t s = 1; s <= std::min<int64_t>(n_tiles, 64); ++s) {
         const int64_t each = ceil_div(n_tiles, s);
-        const int64_t cost = ceil_div(m_tiles * ceil_div(n_tiles, each), sms) * each;
+        const int64_t cost = ceil_div(m_tiles * ceil_div(n_tiles, each), sms) * (4 * each + 1);
         if (cost < best) {
             best = cost;
             span = each;
