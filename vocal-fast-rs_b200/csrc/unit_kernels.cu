@@ -122,12 +122,16 @@ struct Tile {
 // With 6 the tensor cores are a whole tile ahead of the epilogue at depth
 // 768, with 4 they wait for it (forward of 30,000 x 16,384 back to back:
 // 642 us in one run, 658 by 6, 709 by 4).  The backward pass is held up by
-// its epilogue either way and takes 4, which keeps the sums of softmax
-// gradients to 1e-5.  f32 operands, six products a block, take 4 and 2 (2 in
-// the forward pass costs 6%).  Results that are rounded to bf16 take one run.
+// its epilogue either way and takes 4.  f32 operands, six products a block,
+// take 2 and 1: both passes truncate by amounts close to each other, and what
+// they differ by goes into gradients whose sums nearly cancel (64 units,
+// 30,000 rows of 256, errors of dunits and dbias: 3.8e-5 and 4.6e-5 by 4 and
+// 2, 5.2e-5 and 6.5e-5 by 4 and 1, 2.2e-5 and 2.3e-5 by 2 and 1; 4,096 x 4,096
+// x 768 takes 134 us against 128 forward, 384 against 371 backward).  Results
+// that are rounded to bf16 take one run.
 constexpr int kOneRun = 1 << 30;
 template <class S, bool kBackward>
-constexpr int kLogitRun = S::kTerms == 1 ? (kBackward ? 4 : 6) : (kBackward ? 2 : 4);
+constexpr int kLogitRun = S::kTerms == 1 ? (kBackward ? 4 : 6) : (kBackward ? 1 : 2);
 constexpr int kGradientRun = 4;
 
 // A bounded wait of a whole warp, the same answer for every lane.
