@@ -257,6 +257,10 @@ def test_layer_norm_backward_refusals(native, change, message):
 @pytest.mark.parametrize("change,message", [
     (dict(dtype=2), "takes f32 or bf16"),
     (dict(k=0), "unit count must be positive"),
+    # tiles past the last row or unit must keep 32-bit coordinates
+    (dict(k=2 ** 30 + 1), "frames and units must number 2\\^30 at most"),
+    (dict(k=2 ** 31 - 1), "frames and units must number 2\\^30 at most"),
+    (dict(rows=2 ** 30 + 1), "frames and units must number 2\\^30 at most"),
     (dict(width=4097), "row width must be in 1..4096"),
     (dict(scale=float("inf")), "logit scale must be finite"),
     (dict(scale=float("nan")), "logit scale must be finite"),

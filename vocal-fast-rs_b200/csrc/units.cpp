@@ -11,6 +11,9 @@
 namespace vfr {
 namespace {
 
+// Frames and units of the unit loss.  Its kernels hold tile coordinates in 32
+// bits and look up to two tiles of 256 past the last row or unit.
+constexpr int64_t kMaxUnitCount = int64_t(1) << 30;
 
 // The device `p` lives on.  Kernels would fault on host memory, so it is
 // refused; the other arguments are the caller's to keep on the same device.
@@ -50,6 +53,7 @@ void check_units(int64_t rows, int32_t k, int32_t width, int32_t dtype) {
     check_rows(rows, width, dtype);
     require(dtype != kF16, "the unit loss takes f32 or bf16 frames (softmax gradients leave fp16's range)");
     require(k >= 1, "unit count must be positive");
+    require(rows <= kMaxUnitCount && k <= kMaxUnitCount, "frames and units must number 2^30 at most");
 }
 
 cudaStream_t given_stream(const VfrStream *stream) {

@@ -1,7 +1,7 @@
 // Training a content encoder's unit head: layer norm and its gradients, 8-bit
-// activation checkpoints (norm_kernels.cu, checkpoint_kernels.cu), and the softmax cross entropy of
-// frames over a codebook of units with its gradients (unit_kernels.cu).
-// Argument checks and workspace sizes are in units.cpp.
+// activation checkpoints (norm_kernels.cu, checkpoint_kernels.cu), and the
+// softmax cross entropy of frames over a codebook of units with its gradients
+// (unit_kernels.cu).  Argument checks are in units.cpp.
 #pragma once
 
 #include <cuda_runtime.h>

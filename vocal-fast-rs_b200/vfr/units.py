@@ -135,7 +135,8 @@ def checkpoint_pack(x, stream=None) -> Checkpoint:
 
 def checkpoint_unpack(checkpoint: Checkpoint, dtype=None, stream=None):
     """The checkpoint's values, in `dtype` (default: the type it was packed
-    from; float32 holds them exactly)."""
+    from; float32 holds them exactly, but for magnitudes from 1.9375 * 2^127 on,
+    which come out as infinities)."""
     c = _check_checkpoint(checkpoint)
     dtype = c.dtype if dtype is None else dtype
     code = _code(dtype)
