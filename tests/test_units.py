@@ -595,8 +595,10 @@ def _head(torch, rows, k, width, dtype, seed, masked=0):
 UNIT_SHAPES = [(1, 1, 1), (1, 511, 768), (2, 3, 5), (34, 511, 768), (127, 255, 64), (128, 256, 64), (129, 257, 65),
                (140, 504, 256), (300, 1000, 72), (257, 129, 1000), (1000, 33, 8), (5, 2000, 4096), (700, 640, 200),
                (64, 64, 128), (1, 5000, 96), (3000, 2, 16),
-               # large enough for CTA pairs, with ragged last tiles on every side
-               (9001, 4611, 256), (6200, 7000, 450)]
+               # several rounds of tiles, ragged on every side; the gradients'
+               # products of (6200, ...) and below run on CTA pairs in bf16 (a
+               # tile of 256 x 256 for each of 74 pairs at least)
+               (9001, 4611, 256), (6200, 7000, 450), (4500, 4700, 700), (10001, 9001, 770)]
 
 
 @pytest.mark.gpu

@@ -1,6 +1,7 @@
 // 8-bit activation checkpoints: e4m3 with one power of two per 128 elements
-// of a row.  Bound by HBM: packing reads the values and writes a byte each,
-// unpacking the reverse.
+// of a row.  Packing reads the values and writes a byte each, unpacking the
+// reverse.  60,000 x 768: packing f32 39 us (HBM 67% busy), bf16 27 us (46%,
+// instructions issued in 63% of the cycles), unpacking to f32 36 us (59%).
 #include "norm_rows.cuh"
 
 namespace vfr {

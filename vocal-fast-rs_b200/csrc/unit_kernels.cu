@@ -773,6 +773,11 @@ __device__ __forceinline__ void store_gradients(const LogitArgs &a, const CUtens
     __syncwarp();
 }
 
+// Bound by the tensor cores forward (82% busy at 16,384 x 8,192 x 768 bf16,
+// 148 us; f32 76% at 4,096 x 4,096 x 768, 129 us) and, backward, by the
+// epilogue that holds them up (58%, 196 us; f32 63%, 153 us).  Tiles of 128
+// rows keep a row's sums in one lane's registers; single CTAs, as a pair's
+// two epilogues would wait for each other.
 template <class S, bool kBackward>
 __global__ void __launch_bounds__(kThreads, 1)
     logit_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -786,6 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the slots of each row: 32 rows a CTA, a warp for every eighth slot.
+// Bound by latency (16,384 rows: 7 us, 4 MB read).
 __global__ void __launch_bounds__(256) loss_kernel(const float2 *partial, const float *target, const int32_t *labels,
                                                    const float *bias, int64_t rows, int slots, int k, float *loss,
                                                    float *lse) {
@@ -896,6 +902,9 @@ struct ProductWalk {
     }
 };
 
+// Bound by the tensor cores: 95% busy by pairs (16,384 x 8,192 x 768 bf16,
+// both products 287 us, 1,435 TFLOP/s), 78% in f32 (4,096 x 4,096 x 768, 250
+// us, six products each).
 template <class S>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_gt,
@@ -1031,6 +1040,8 @@ __global__ void __launch_bounds__(kFinishThreads) finish_kernel(const FinishArgs
 // The products' operands: rows of bf16 terms, padded with zeros to 64 columns.
 // With `clean`, frames without a label and units left out become zero rows:
 // a zero of G times an infinity or a NaN there would reach the gradients.
+// A warp a row, each element once (24,576 rows of 768 bf16: 14 us, a third of
+// HBM's rate).
 struct StageArgs {
     const void *x, *units;
     const float *bias;
@@ -1180,11 +1191,14 @@ int tile_columns(int64_t m_tiles, int64_t cols, int terms, int sms) {
     return best;
 }
 
-// Whether CTA pairs serve a product of so many rows and columns: full tiles
-// of 256 by 256 for two rounds of the pairs at least, and less than a quarter
-// of the columns' tiles empty.
+// Whether CTA pairs serve a product of so many rows and columns: a tile of 256
+// by 256 for every pair at least, and less than a quarter of the columns'
+// tiles empty.  Gradients, width 768, bf16, with pairs and without: 30,000 x
+// 16,384 1,723 us and 1,956, 8,192^2 251 and 300, 8,192 x 4,096 140 and 161,
+// 5,120^2 122 and 134, 3,500^2 (84 tiles) 101 and 99; below a tile a pair,
+// 3,200 x 2,900 (72 tiles) 91 and 67.
 bool pairs_fit(int64_t rows, int64_t cols, int terms, int sms) {
-    return terms == 1 && ceil_div(rows, 256) * ceil_div(cols, 256) >= sms && ceil_div(cols, 256) * 192 <= cols;
+    return terms == 1 && ceil_div(rows, 256) * ceil_div(cols, 256) >= sms / 2 && ceil_div(cols, 256) * 192 <= cols;
 }
 
 // Column tiles of an item: the shortest rounds of the grid, an item costing a
